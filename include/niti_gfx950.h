@@ -579,6 +579,44 @@ int niti_head_i8_backward_unpool(const int8_t* err, const int8_t* act, const int
 int niti_group_conv_i8_f32(const int8_t* x, const int8_t* w, float* y, int N, int H, int W, int C, int K, int R,
                            int S, int Cg, int stride, int pad, int dilation, int groups, void* stream);
 
+/*
+ * Losses over many classes, the logits kept nowhere.  No counterpart in the reference, whose loss (ti_loss.py:5-36) takes int8
+ * logits that lie in memory.  act: [rows][features] int8, w: [classes][features] int8, rows act_pitch / w_pitch bytes apart (any
+ * alignment; multiples of 16 bytes throughout are read in place), exponents in device memory; a logit is
+ * z = (act . w) 2^(exp_a + exp_w), the sum exact in int32 (features <= 65536).
+ *
+ * niti_vocab_entropy_i8: loss[n] = log sum_v exp(z[n,v]) - z[n,target[n]], lse[n] = log sum_v exp(z[n,v]) in float32.  target: int32
+ * or int64 by target_bytes.  A row whose target is `ignored` has loss 0 and no gradient; any other target outside the classes
+ * makes the row's loss and all gradients that it has part in NaN.
+ *
+ * niti_vocab_distill_i8: against a teacher's `top` (<= 1024) best logits per row, top_value (float32, bfloat16 or float16 by value_type) at
+ * top_class; a negative class is an unused place, one beyond the classes makes the row NaN as above.  With z' = z / T and
+ * q = softmax(top_value / T) over a row's used places, lse of z':
+ *   loss[n] = T^2 sum_j q_j (log q_j - (z'[n, class_j] - lse[n]))
+ * A row without used places, or whose values are all -inf, has loss 0 and no gradient.  A class may be named more than once.
+ *
+ * Both leave in `state` (rows * niti_vocab_state_words(top) int32, 16-byte aligned; top = 1 for the entropy) what niti_vocab_backward_i8 needs: gradients
+ * of sum_n weight[n] loss[n] with respect to act 2^exp_a (d_act [rows][features]) and w 2^exp_w (d_w [classes][features]) as bfloat16, from
+ * sums in float32.  weight: `weights` = rows values, one for all, or null for 1.  The logits are computed again, a piece of the
+ * classes at a time; the softmax of a piece is held as float16 times 2^15.
+ *
+ * The workspaces depend on the operands' addresses through their alignment alone.
+ */
+enum { NITI_F32 = 0, NITI_BF16 = 1, NITI_F16 = 2 };
+size_t niti_vocab_state_words(int top);
+size_t niti_vocab_forward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes);
+size_t niti_vocab_backward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes);
+int niti_vocab_entropy_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w,
+                          int rows, int features, int classes, const void* target, int target_bytes, int64_t ignored, float* loss, float* lse,
+                          int32_t* state, void* workspace, size_t workspace_bytes, void* stream);
+int niti_vocab_distill_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w,
+                          int rows, int features, int classes, const void* top_value, int value_type, const void* top_class, int class_bytes,
+                          int top, float temperature, float* loss, float* lse, int32_t* state, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w,
+                           int rows, int features, int classes, int top, float temperature, const int32_t* state, const float* weight,
+                           int weights, uint16_t* d_act, uint16_t* d_w, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ==================================================================================================================
  * MEASUREMENT ONLY - not part of the boundary a reference checkout binds to; nothing in the layers calls it.
  * ================================================================================================================== */

@@ -402,7 +402,8 @@ at::Tensor scratch(size_t bytes, const at::Tensor& like) {
 PyMODINIT_FUNC PyInit__host() {
   PyObject* m = PyModule_Create(&niti_host::kModule);
   if (m == nullptr) return nullptr;
-  if (PyModule_AddFunctions(m, niti_host::kConvMethods) != 0 || PyModule_AddFunctions(m, niti_host::kLinearMethods) != 0) {
+  if (PyModule_AddFunctions(m, niti_host::kConvMethods) != 0 || PyModule_AddFunctions(m, niti_host::kLinearMethods) != 0 ||
+      PyModule_AddFunctions(m, niti_host::kVocabMethods) != 0) {
     Py_DECREF(m);
     return nullptr;
   }

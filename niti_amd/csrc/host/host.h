@@ -1,4 +1,4 @@
-// Helpers of the tensor front end (host.cpp, conv.cpp, linear.cpp): argument access, allocation, error reporting.
+// Helpers of the tensor front end (host.cpp, conv.cpp, linear.cpp, vocab.cpp): argument access, allocation, error reporting.
 //
 // The front end is the part of niti_amd/ops.py that runs on every call - argument checks, output allocation, sync words,
 // the call into the C ABI - as native code.  A launch takes the GPU 5 - 20 us at the sizes of a layer; the same steps in
@@ -63,6 +63,18 @@ class Args {
     Opt t = opt();
     if (t != nullptr && (t->numel() != 1 || t->scalar_type() != at::kInt)) refuse("niti_amd: an exponent is one int32 value");
     return t;
+  }
+  const at::Tensor& strided() {   // any strides: the caller looks at them
+    PyObject* o = a_[i_++];
+    if (!THPVariable_Check(o)) refuse("niti_amd: tensor expected");
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda()) refuse("niti_amd: tensor must live on the GPU");
+    return t;
+  }
+  double number() {
+    const double v = PyFloat_AsDouble(a_[i_++]);
+    if (v == -1.0 && PyErr_Occurred()) throw python_error();
+    return v;
   }
   long integer() {
     const long v = PyLong_AsLong(a_[i_++]);
@@ -161,5 +173,6 @@ inline PyObject* guarded(F f) {
 // tables of the other translation units
 extern PyMethodDef kConvMethods[];
 extern PyMethodDef kLinearMethods[];
+extern PyMethodDef kVocabMethods[];
 
 }  // namespace niti_host

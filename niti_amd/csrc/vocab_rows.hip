@@ -1,0 +1,471 @@
+// Losses over a large vocabulary (vocab.h): what is done per row, the operands' layouts, and the entry points.
+//
+//   forward:  statistics of the logits per row and kVocabClassTile classes (vocab.hip), then a wavefront per row joins them, multiplies out the logits
+//             of the row's targets, and leaves loss, logarithm of the denominator and what the backward pass wants to know
+//   backward: a piece of the classes after the other: the piece's softmax as 16-bit floats (vocab.hip), the targets' places
+//             overwritten with their gradient (known in 32 bits: a small difference p - q keeps its digits), both products
+#include <math.h>
+
+#include "vocab.h"
+
+namespace niti {
+namespace {
+
+constexpr int kMaxFeatures = 65536;      // |s| <= 2^30: differences of two logits are int32
+constexpr long long kPieceMost = 1LL << 20;
+constexpr long long kPieceGrad = 64LL << 20;    // elements of the gradient's piece
+constexpr long long kPieceWide = 128LL << 20;   // elements of the weights' 16-bit piece
+
+long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
+
+// ---- layouts -------------------------------------------------------------------------------------------------------
+// rows of `n` bytes at any address and pitch -> rows of a multiple of 16, zero behind the last byte
+__global__ __launch_bounds__(256) void vocab_pad_kernel(const int8_t* __restrict__ src, long long pitch, int8_t* __restrict__ dst, long long rows, int n) {
+  const int pieces = (n + 15) / 16;
+  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= rows * pieces) return;
+  const long long row = at / pieces;
+  const int c = static_cast<int>(at - row * pieces) * 16;
+  union {
+    int8_t b[16];
+    v4i v;
+  } u;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) u.b[i] = c + i < n ? src[row * pitch + c + i] : static_cast<int8_t>(0);
+  *reinterpret_cast<v4i*>(dst + at * 16) = u.v;
+}
+
+// int8 rows (16-byte aligned, `n` values, zero up to the next multiple of 16) -> 16-bit floats, times weight / 2^*exponent 2^kRowExponent
+// of the row where there are weights
+__global__ __launch_bounds__(256) void vocab_widen_kernel(const int8_t* __restrict__ src, long long src_pitch, _Float16* __restrict__ dst, long long pitch,
+                                                          long long rows, int n, const float* __restrict__ weight, const int32_t* __restrict__ exponent) {
+  const int pieces = (n + 15) / 16;
+  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= rows * pieces) return;
+  const long long row = at / pieces;
+  const int c = static_cast<int>(at - row * pieces) * 16;
+  union {
+    int8_t b[16];
+    v4i v;
+  } u;
+  u.v = *reinterpret_cast<const v4i*>(src + row * src_pitch + c);
+  float scale = 1.0f;
+  if (weight != nullptr) scale = ldexpf(weight[row], kRowExponent - *exponent);
+  _Float16 o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = static_cast<_Float16>(static_cast<float>(u.b[i]) * scale);
+  v4i* const out = reinterpret_cast<v4i*>(dst + row * pitch + c);
+  out[0] = *reinterpret_cast<v4i*>(&o[0]);
+  out[1] = *reinterpret_cast<v4i*>(&o[8]);
+}
+
+// smallest power of two above every weight's magnitude, as an exponent; one workgroup
+__global__ __launch_bounds__(1024) void vocab_weight_exponent_kernel(const float* __restrict__ weight, int n, int32_t* __restrict__ exponent) {
+  __shared__ float most[16];
+  float m = 0.0f;
+  for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, fabsf(weight[i]));
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) m = fmaxf(m, most[i]);
+    int e = 0;
+    if (m > 0.0f) frexpf(fminf(m, 3.402823466e38f), &e);
+    *exponent = e;
+  }
+}
+
+// ---- rows ------------------------------------------------------------------------------------------------------------
+struct VocabRows {
+  const int2* part;           // [rows][tiles]
+  int tiles;
+  const int8_t* a;            // 16-byte aligned rows, zero behind the features
+  const int8_t* w;
+  long long a_pitch, w_pitch;
+  int rows, classes, pieces;  // pieces of 16 features
+  const int32_t* exp_a;
+  const int32_t* exp_w;
+  float t;
+  const void* index;          // [rows][top]
+  int index_bytes;
+  long long ignored;          // entropy: this class is none; distillation: every negative one
+  const void* value;          // [rows][top] teacher's logits; null: entropy
+  int value_type;
+  int top;
+  float* loss;
+  float* lse;
+  int32_t* state;
+};
+
+__device__ inline float teacher_value(const VocabRows& a, long long i) {
+  if (a.value_type == NITI_F32) return static_cast<const float*>(a.value)[i];
+  if (a.value_type == NITI_BF16) return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(a.value)[i]) << 16);
+  return static_cast<float>(static_cast<const _Float16*>(a.value)[i]);
+}
+
+__device__ inline double wave_sum(double v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// A wavefront per row.  All lanes go through every loop the same number of times: the barriers are the workgroup's.
+__global__ __launch_bounds__(256) void vocab_rows_kernel(const VocabRows a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const bool real = blockIdx.x * 4 + wave < static_cast<unsigned>(a.rows);
+  const long long row = real ? blockIdx.x * 4 + wave : a.rows - 1;
+  float* const q = reinterpret_cast<float*>(smem) + wave * 3 * a.top;
+  int* const cls = reinterpret_cast<int*>(q + a.top);
+  int* const dot = cls + a.top;
+  const double k = fmin(ldexp(1.4426950408889634074 / static_cast<double>(a.t), *a.exp_a + *a.exp_w), 3.402823466e38);
+  const float kf = static_cast<float>(k);
+
+  const int2* const part = a.part + row * a.tiles;
+  int m = -2147483647 - 1;
+  for (int i = lane; i < a.tiles; i += 64) m = max(m, part[i].x);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) m = max(m, __shfl_xor(m, off, 64));
+  double sum = 0.0;
+  for (int i = lane; i < a.tiles; i += 64) {
+    const int2 v = part[i];
+    sum += static_cast<double>(__int_as_float(v.y) * exp2f(static_cast<float>(v.x - m) * kf));
+  }
+  const double l2 = log2(wave_sum(sum));
+
+  // the targets and their weights
+  bool bad = false;
+  float vmax = -INFINITY;
+  for (int j = lane; j < a.top; j += 64) {
+    const long long at = row * a.top + j;
+    const long long c = a.index_bytes == 8 ? static_cast<const int64_t*>(a.index)[at] : static_cast<const int32_t*>(a.index)[at];
+    const bool none = a.value == nullptr ? c == a.ignored : c < 0;
+    if (!none && (c < 0 || c >= a.classes)) bad = true;
+    const bool used = !none && c >= 0 && c < a.classes;
+    cls[j] = used ? static_cast<int>(c) : -1;
+    const float v = !used ? -INFINITY : (a.value == nullptr ? 0.0f : teacher_value(a, at) / a.t);
+    q[j] = v;
+    vmax = fmaxf(vmax, v);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, off, 64));
+  bad = __any(bad);
+  double norm = 0.0;
+  for (int j = lane; j < a.top; j += 64) {
+    const float v = q[j];
+    const float e = v == -INFINITY ? 0.0f : expf(v - vmax);
+    q[j] = e;
+    norm += static_cast<double>(e);
+  }
+  norm = wave_sum(norm);
+  const float coef = bad ? __builtin_nanf("") : (norm > 0.0 ? 1.0f : (norm == 0.0 ? 0.0f : __builtin_nanf("")));
+  __syncthreads();
+
+  // the targets' logits, four at a time
+  const v4i* const arow = reinterpret_cast<const v4i*>(a.a + row * a.a_pitch);
+  for (int j0 = 0; j0 < a.top; j0 += 4) {
+    int s[4] = {0, 0, 0, 0};
+    const v4i* w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = j0 + u < a.top ? cls[j0 + u] : -1;
+      w[u] = reinterpret_cast<const v4i*>(a.w + (c < 0 ? 0 : c) * a.w_pitch);   // an unused place's product is not looked at
+    }
+    for (int p = lane; p < a.pieces; p += 64) {
+      const v4i x = arow[p];
+      v4i y[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) y[u] = w[u][p];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u] = __builtin_amdgcn_sdot4(x[i], y[u][i], s[u], false);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) s[u] += __shfl_xor(s[u], off, 64);
+      if (lane == 0 && j0 + u < a.top) dot[j0 + u] = s[u];
+    }
+  }
+  __syncthreads();
+
+  constexpr double kLn2 = 0.69314718055994530942;
+  int32_t* const state = a.state + row * vocab_state_words(a.top);
+  double loss = 0.0;
+  for (int j = lane; j < a.top; j += 64) {
+    const int c = cls[j];
+    float g = 0.0f;
+    bool first = c >= 0;
+    if (c >= 0) {
+      const double mine = static_cast<double>(q[j]) / norm;
+      if (mine > 0.0) loss += mine * (log(mine) + kLn2 * (l2 + (static_cast<double>(m) - dot[j]) * k));
+      else if (!(mine == 0.0)) loss = mine;
+      float all = 0.0f;                  // the weights of every place that names this class
+      for (int i = 0; i < a.top; ++i)
+        if (cls[i] == c) {
+          all += q[i];
+          if (i < j) first = false;      // one place speaks for all
+        }
+      const float p = exp2f(static_cast<float>((static_cast<double>(dot[j]) - m) * k - l2));
+      g = norm > 0.0 ? p - static_cast<float>(static_cast<double>(all) / norm) : 0.0f;
+      if (coef != coef) g = coef;
+    }
+    if (real) {
+      state[4 + 2 * j] = __float_as_int(g);
+      state[5 + 2 * j] = first ? c : -1;
+    }
+  }
+  loss = wave_sum(loss) * a.t * a.t;
+  if (lane == 0 && real) {
+    a.loss[row] = norm == 0.0 && !bad ? 0.0f : (coef != coef ? coef : static_cast<float>(loss));
+    a.lse[row] = static_cast<float>(kLn2 * (l2 + m * k));
+    *reinterpret_cast<v4i*>(state) = v4i{m, __float_as_int(static_cast<float>(l2)), __float_as_int(coef), 0};
+  }
+}
+
+// the targets' gradients into a piece of the softmax
+__global__ __launch_bounds__(256) void vocab_targets_kernel(const int32_t* __restrict__ state, int rows, int top, long long first, int classes,
+                                                            _Float16* __restrict__ g, long long pitch) {
+  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= static_cast<long long>(rows) * top) return;
+  const long long row = at / top;
+  const int32_t* const s = state + row * vocab_state_words(top) + 4 + 2 * (at - row * top);
+  const long long c = s[1] - first;
+  if (s[1] >= 0 && c >= 0 && c < classes) g[row * pitch + c] = static_cast<_Float16>(ldexpf(__int_as_float(s[0]), kGradExponent));
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+struct Matrix {      // as the caller has it
+  const int8_t* p;
+  long long pitch;
+  long long rows;
+};
+// the products read 16 bytes at a time, whole rows of them
+bool needs_copy(const Matrix& m, int features) { return ((reinterpret_cast<uintptr_t>(m.p) | static_cast<uintptr_t>(m.pitch) | static_cast<uintptr_t>(features)) & 15) != 0; }
+
+struct Layout {
+  size_t bytes = 0;
+  size_t take(long long n) {
+    const size_t at = bytes;
+    bytes += static_cast<size_t>(round_up(n, 256));
+    return at;
+  }
+};
+
+struct ForwardPlan {
+  size_t a, w, part, bytes;
+  bool copy_a, copy_w;
+  int tiles;
+};
+ForwardPlan forward_plan(const Matrix& a, const Matrix& w, int features) {
+  ForwardPlan p{};
+  Layout l;
+  const long long row = round_up(features, 16);
+  p.copy_a = needs_copy(a, features);
+  p.copy_w = needs_copy(w, features);
+  p.a = l.take(p.copy_a ? a.rows * row : 0);
+  p.w = l.take(p.copy_w ? w.rows * row : 0);
+  p.tiles = static_cast<int>((w.rows + kVocabClassTile - 1) / kVocabClassTile);
+  p.part = l.take(a.rows * p.tiles * 8);
+  p.bytes = l.bytes;
+  return p;
+}
+
+struct BackwardPlan {
+  size_t a, w, wide_a, wide_w, grad, part_a, part_w, exponent, bytes;
+  bool copy_a, copy_w;
+  long long piece, pitch16, part_pitch;   // classes at a time; values of a 16-bit row; values of a partial sum's row
+  int slices_a, steps_a, slices_w, steps_w;
+  bool parts_a, parts_w;
+};
+BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
+  BackwardPlan p{};
+  Layout l;
+  const long long row = round_up(features, 16);
+  p.copy_a = needs_copy(a, features);
+  p.copy_w = needs_copy(w, features);
+  p.pitch16 = row;
+  p.part_pitch = round_up(features, 4);
+  long long piece = kPieceGrad / a.rows;
+  if (piece > kPieceWide / features) piece = kPieceWide / features;
+  if (piece < 4096) piece = 4096;
+  if (piece > kPieceMost) piece = kPieceMost;
+  piece = piece / kVocabClassTile * kVocabClassTile;
+  if (piece > round_up(w.rows, 8)) piece = round_up(w.rows, 8);
+  p.piece = piece;
+  vocab_sums_plan(features, static_cast<int>(a.rows), static_cast<int>(piece), &p.slices_a, &p.steps_a);
+  vocab_sums_plan(features, static_cast<int>(piece), static_cast<int>(a.rows), &p.slices_w, &p.steps_w);
+  p.parts_a = p.slices_a > 1 || piece < w.rows;
+  p.parts_w = p.slices_w > 1;
+  p.a = l.take(p.copy_a ? a.rows * row : 0);
+  p.w = l.take(p.copy_w ? w.rows * row : 0);
+  p.wide_a = l.take(a.rows * p.pitch16 * 2);
+  p.wide_w = l.take(piece * p.pitch16 * 2);
+  p.grad = l.take(a.rows * piece * 2);
+  p.part_a = l.take(p.parts_a ? p.slices_a * a.rows * p.part_pitch * 4 : 0);
+  p.part_w = l.take(p.parts_w ? p.slices_w * piece * p.part_pitch * 4 : 0);
+  p.exponent = l.take(4);
+  p.bytes = l.bytes;
+  return p;
+}
+
+int pad_rows(const Matrix& m, int features, int8_t* dst, hipStream_t stream) {
+  const long long n = m.rows * ((features + 15) / 16);
+  hipLaunchKernelGGL(vocab_pad_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, stream, m.p, m.pitch, dst, m.rows, features);
+  return check_launch("vocab_pad");
+}
+int widen_rows(const Matrix& m, int features, _Float16* dst, long long pitch, const float* weight, const int32_t* exponent, hipStream_t stream) {
+  const long long n = m.rows * ((features + 15) / 16);
+  hipLaunchKernelGGL(vocab_widen_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, stream, m.p, m.pitch, dst, pitch, m.rows, features, weight,
+                     exponent);
+  return check_launch("vocab_widen");
+}
+VocabOperand bytes_operand(const Matrix& m, int features) {
+  return VocabOperand{m.p, m.pitch, static_cast<int>(m.rows), static_cast<int>(round_up(features, 16))};
+}
+
+int check_operands(const char* who, const int8_t* act, long long act_pitch, const int8_t* w, long long w_pitch, const int32_t* exp_a, const int32_t* exp_w,
+                   int rows, int features, int classes, int top) {
+  if (act == nullptr || w == nullptr || exp_a == nullptr || exp_w == nullptr) return fail(NITI_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (rows <= 0 || features <= 0 || classes <= 0 || top <= 0)
+    return fail(NITI_ERR_INVALID_ARG, "%s: rows=%d features=%d classes=%d top=%d", who, rows, features, classes, top);
+  if (act_pitch < features || w_pitch < features) return fail(NITI_ERR_INVALID_ARG, "%s: rows of %lld and %lld bytes hold no %d features", who, act_pitch, w_pitch, features);
+  if (features > kMaxFeatures) return fail(NITI_ERR_UNSUPPORTED, "%s: %d features (at most %d)", who, features, kMaxFeatures);
+  if (act_pitch >= (1LL << 22) || w_pitch >= (1LL << 22)) return fail(NITI_ERR_UNSUPPORTED, "%s: rows 4 MiB or more apart", who);
+  if (top > kVocabTopMost) return fail(NITI_ERR_UNSUPPORTED, "%s: lists of %d (at most %d)", who, top, kVocabTopMost);
+  return NITI_OK;
+}
+
+int forward(const char* who, const int8_t* act, long long act_pitch, const int8_t* w, long long w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+            int features, int classes, const void* value, int value_type, const void* index, int index_bytes, long long ignored, int top, float t, float* loss,
+            float* lse, int32_t* state, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (const int rc = check_operands(who, act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top)) return rc;
+  if (index == nullptr || loss == nullptr || lse == nullptr || state == nullptr) return fail(NITI_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (index_bytes != 4 && index_bytes != 8) return fail(NITI_ERR_INVALID_ARG, "%s: classes of %d bytes (4 or 8)", who, index_bytes);
+  if (!aligned16(state)) return fail(NITI_ERR_INVALID_ARG, "%s: state not 16-byte aligned", who);
+  Matrix a{act, act_pitch, rows}, b{w, w_pitch, classes};
+  const ForwardPlan p = forward_plan(a, b, features);
+  if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
+    return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
+  char* const ws = static_cast<char*>(workspace);
+  if (p.copy_a) {
+    if (const int rc = pad_rows(a, features, reinterpret_cast<int8_t*>(ws + p.a), stream)) return rc;
+    a = Matrix{reinterpret_cast<int8_t*>(ws + p.a), round_up(features, 16), rows};
+  }
+  if (p.copy_w) {
+    if (const int rc = pad_rows(b, features, reinterpret_cast<int8_t*>(ws + p.w), stream)) return rc;
+    b = Matrix{reinterpret_cast<int8_t*>(ws + p.w), round_up(features, 16), classes};
+  }
+  int2* const part = reinterpret_cast<int2*>(ws + p.part);
+  const VocabLogits l{bytes_operand(b, features), bytes_operand(a, features), classes, rows, features, exp_a, exp_w, 1.0f / t};
+  if (const int rc = launch_vocab_stats(l, VocabStats{part, p.tiles}, stream)) return rc;
+  const VocabRows r{part, p.tiles, a.p, b.p, a.pitch, b.pitch, rows, classes, (features + 15) / 16, exp_a, exp_w, t, index, index_bytes, ignored, value, value_type,
+                    top, loss, lse, state};
+  hipLaunchKernelGGL(vocab_rows_kernel, dim3((rows + 3) / 4), dim3(256), 4 * 12 * top, stream, r);
+  return check_launch(who);
+}
+
+}  // namespace
+}  // namespace niti
+
+using namespace niti;
+
+extern "C" size_t niti_vocab_state_words(int top) { return top > 0 ? static_cast<size_t>(vocab_state_words(top)) : 0; }
+
+extern "C" size_t niti_vocab_forward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
+  if (rows <= 0 || features <= 0 || classes <= 0) return 0;
+  return forward_plan(Matrix{act, act_pitch, rows}, Matrix{w, w_pitch, classes}, features).bytes;
+}
+
+extern "C" size_t niti_vocab_backward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
+  if (rows <= 0 || features <= 0 || classes <= 0) return 0;
+  return backward_plan(Matrix{act, act_pitch, rows}, Matrix{w, w_pitch, classes}, features).bytes;
+}
+
+extern "C" int niti_vocab_entropy_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                                     int features, int classes, const void* target, int target_bytes, int64_t ignored, float* loss, float* lse, int32_t* state,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  return forward("vocab_entropy", act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, nullptr, 0, target, target_bytes, ignored, 1, 1.0f, loss, lse,
+                 state, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int niti_vocab_distill_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                                     int features, int classes, const void* top_value, int value_type, const void* top_class, int class_bytes, int top,
+                                     float temperature, float* loss, float* lse, int32_t* state, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (top_value == nullptr) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: null pointer");
+  if (value_type != NITI_F32 && value_type != NITI_BF16 && value_type != NITI_F16) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: value_type=%d", value_type);
+  if (!(temperature > 0.0f) || !isfinite(temperature)) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: temperature %g", static_cast<double>(temperature));
+  return forward("vocab_distill", act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top_value, value_type, top_class, class_bytes, -1, top, temperature,
+                 loss, lse, state, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                                      int features, int classes, int top, float temperature, const int32_t* state, const float* weight, int weights,
+                                      uint16_t* d_act, uint16_t* d_w, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const char* const who = "vocab_backward";
+  hipStream_t const st = static_cast<hipStream_t>(stream);
+  if (const int rc = check_operands(who, act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top)) return rc;
+  if (state == nullptr || d_act == nullptr || d_w == nullptr) return fail(NITI_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (weight != nullptr && weights != 1 && weights != rows) return fail(NITI_ERR_INVALID_ARG, "%s: %d weights for %d rows", who, weights, rows);
+  if (!(temperature > 0.0f) || !isfinite(temperature)) return fail(NITI_ERR_INVALID_ARG, "%s: temperature %g", who, static_cast<double>(temperature));
+  if (!aligned16(state) || !aligned16(d_act) || !aligned16(d_w)) return fail(NITI_ERR_INVALID_ARG, "%s: state or result not 16-byte aligned", who);
+  Matrix a{act, act_pitch, rows}, b{w, w_pitch, classes};
+  const BackwardPlan p = backward_plan(a, b, features);
+  if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
+    return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
+  char* const ws = static_cast<char*>(workspace);
+  if (p.copy_a) {
+    if (const int rc = pad_rows(a, features, reinterpret_cast<int8_t*>(ws + p.a), st)) return rc;
+    a = Matrix{reinterpret_cast<int8_t*>(ws + p.a), round_up(features, 16), rows};
+  }
+  if (p.copy_w) {
+    if (const int rc = pad_rows(b, features, reinterpret_cast<int8_t*>(ws + p.w), st)) return rc;
+    b = Matrix{reinterpret_cast<int8_t*>(ws + p.w), round_up(features, 16), classes};
+  }
+  _Float16* const wide_a = reinterpret_cast<_Float16*>(ws + p.wide_a);
+  _Float16* const wide_w = reinterpret_cast<_Float16*>(ws + p.wide_w);
+  _Float16* const grad = reinterpret_cast<_Float16*>(ws + p.grad);
+  int32_t* const exponent = reinterpret_cast<int32_t*>(ws + p.exponent);
+  // weights of the rows go into the activations' 16-bit copy (their sum over the rows is one product); one weight for all into the result
+  const bool each = weight != nullptr && weights == rows && rows > 1;
+  if (each) {
+    hipLaunchKernelGGL(vocab_weight_exponent_kernel, dim3(1), dim3(1024), 0, st, weight, rows, exponent);
+    if (const int rc = check_launch(who)) return rc;
+  }
+  if (const int rc = widen_rows(a, features, wide_a, p.pitch16, each ? weight : nullptr, exponent, st)) return rc;
+
+  for (long long first = 0; first < classes; first += p.piece) {
+    const int here = static_cast<int>(classes - first < p.piece ? classes - first : p.piece);
+    const Matrix piece{b.p + first * b.pitch, b.pitch, here};
+    if (const int rc = widen_rows(piece, features, wide_w, p.pitch16, nullptr, nullptr, st)) return rc;
+    const VocabLogits l{bytes_operand(piece, features), bytes_operand(a, features), here, rows, features, exp_a, exp_w, 1.0f / temperature};
+    if (const int rc = launch_vocab_grad(l, VocabGrad{state, vocab_state_words(top), grad, p.piece}, st)) return rc;
+    const long long places = static_cast<long long>(rows) * top;
+    hipLaunchKernelGGL(vocab_targets_kernel, dim3(static_cast<unsigned>((places + 255) / 256)), dim3(256), 0, st, state, rows, top, first, here, grad, p.piece);
+    if (const int rc = check_launch(who)) return rc;
+
+    const int stages = (here + 63) / 64;
+    VocabSums sa{VocabOperand{wide_w, p.pitch16 * 2, here, 0}, VocabOperand{grad, p.piece * 2, rows, static_cast<int>(round_up(here, 8) * 2)}, features, rows, here,
+                 (stages + p.steps_a - 1) / p.steps_a, p.steps_a, p.parts_a ? reinterpret_cast<float*>(ws + p.part_a) : nullptr, p.part_pitch, first > 0 ? 1 : 0, d_act,
+                 temperature, exp_w, -kGradExponent, nullptr, weight, weights};
+    if (const int rc = launch_vocab_sums(sa, false, st)) return rc;
+    VocabSums sw{VocabOperand{wide_a, p.pitch16 * 2, rows, 0}, VocabOperand{grad, p.piece * 2, rows, 0}, features, here, rows, p.slices_w, p.steps_w,
+                 p.parts_w ? reinterpret_cast<float*>(ws + p.part_w) : nullptr, p.part_pitch, 0, d_w + first * features, temperature, exp_a,
+                 -kGradExponent - (each ? kRowExponent : 0), each ? exponent : nullptr, each ? nullptr : weight, 1};
+    if (const int rc = launch_vocab_sums(sw, true, st)) return rc;
+    if (p.parts_w) {
+      if (const int rc = launch_vocab_join(sw, st)) return rc;
+    }
+    if (p.parts_a && first + p.piece >= classes) {
+      sa.slices = p.slices_a;
+      if (const int rc = launch_vocab_join(sa, st)) return rc;
+    }
+  }
+  return NITI_OK;
+}

@@ -338,6 +338,41 @@ def batch_metrics(out_val, out_exp, target, sums):
             "niti_batch_metrics_i8")
 
 
+class VocabState:
+    """What a forward call of vocab_loss / vocab_distill leaves for vocab_backward: per row the logits' maximum, the logarithm of the
+    softmax's denominator and the gradient at the row's targets."""
+    __slots__ = ("rows", "top", "temperature")
+
+    def __init__(self, rows, top, temperature):
+        self.rows, self.top, self.temperature = rows, top, temperature
+
+
+def vocab_loss(act, w, exp_a, exp_w, target, ignore_index=-100):
+    """Softmax cross entropy of a classifier over many classes, its logits kept nowhere: act [..., F] int8, w [V,F] int8, exponents
+    as 1-element int32 tensors, z = (act @ w^T) 2^(exp_a + exp_w).  target [...] int64 or int32; ``ignore_index``: no target, the
+    row's loss is 0 and it has no gradient; any other target outside the classes makes the row's loss (and the gradients) NaN.  Rows
+    may be spaced apart (a slice of a wider tensor).  Returns (loss [...], log sum exp z [...], state), float32, one per row."""
+    loss, lse, rows = L.host().vocab_forward(act, w, exp_a, exp_w, None, target, ignore_index, 1.0)
+    return loss, lse, VocabState(rows, 1, 1.0)
+
+
+def vocab_distill(act, w, exp_a, exp_w, top_val, top_idx, temperature=1.0):
+    """The same classifier against a teacher's top logits: top_val [..., K] (float32, bfloat16 or float16) at the classes top_idx [..., K]
+    (int64 or int32; a negative one is an unused place, one beyond the classes makes the row NaN; K <= 1024).  With
+    q = softmax(top_val / T) over a row's used places and p = softmax(z / T) over all classes, loss = T^2 sum q (log q - log p); a
+    row without used places has loss 0 and no gradient.  Returns (loss [...], log sum exp (z / T) [...], state)."""
+    loss, lse, rows = L.host().vocab_forward(act, w, exp_a, exp_w, top_val, top_idx, 0, temperature)
+    return loss, lse, VocabState(rows, top_idx.shape[-1], temperature)
+
+
+def vocab_backward(act, w, exp_a, exp_w, state, grad=None):
+    """Gradients of sum(grad * loss) of the vocab_loss or vocab_distill call that returned ``state``, with respect to the real values
+    act 2^exp_a and w 2^exp_w: (d_act like act, d_w [V,F]) as bfloat16, summed in float32.  ``grad``: float32, one value or one per
+    row; None: 1.  The softmax is computed again, a piece of the classes at a time, and held as float16 (scaled: eleven bits down
+    to 2^-29), so the gradients carry two roundings more than the sums: that of p - q to eleven bits, and the result's to eight."""
+    return L.host().vocab_backward(act, w, exp_a, exp_w, state.rows, state.top, state.temperature, grad)
+
+
 def mask_features(x, mask, exp_in=None, exp_add=None):
     """x [rows, F] int8 times a keep / drop byte per feature (mask [F] int8 0/1) in one launch.  With ``exp_add`` also
     returns a 1-element int32 tensor holding exp_in + exp_add."""
