@@ -22,6 +22,8 @@ struct Tile {
   static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
   static constexpr int BI = TI / WI / 16, BJ = TJ / WJ / 16;   // 16 x 16 blocks of a wavefront
   static constexpr int kLds = 2 * (TI + TJ) * kStageBytes;
+  // workgroups per unit that the registers are cut for: two wavefronts per SIMD at least, so that all sums are ordinary registers
+  static constexpr int kPerUnit = kWaves >= 8 ? 1 : 8 / kWaves;
 };
 typedef Tile<256, 256, 2, 4> TileLarge;
 typedef Tile<128, 128, 2, 2> TileMiddle;
@@ -93,25 +95,29 @@ struct Source {
     }
   }
 
-  __device__ void issue(unsigned lds) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the stage that load() fetches instructions of; next() moves on
+  __device__ __amdgpu_buffer_rsrc_t stage() const {
     const int n = left <= 0 ? 0 : (left > 0x7fffffffLL ? 0x7fffffff : static_cast<int>(left));
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, n, 0x00020000);
-    const bool in = kSlow || piece < fast_left;
-#pragma unroll
-    for (int q = 0; q < kLoads; ++q)
-      if (kInstructions >= kWaves || wave < kInstructions) __builtin_amdgcn_raw_ptr_buffer_load_lds(r, NITI_LDS_AT(lds + (q * kWaves + wave) * 1024), 16, in ? voff[q] : kFar, 0, 0, 0);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, n, 0x00020000);
+  }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned lds, int q) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (kInstructions >= kWaves || wave < kInstructions)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, NITI_LDS_AT(lds + (q * kWaves + wave) * 1024), 16, kSlow || piece < fast_left ? voff[q] : kFar, 0, 0, 0);
+  }
+  __device__ void next() {
     base += advance;
     left -= advance;
     fast_left -= kStageBytes;
   }
 };
 
-// Fragment reads of B blocks of 16 rows / columns, starting at block `first` of the operand's stage at LDS address `lds`.
+// Fragment reads of B blocks of 16 rows / columns, starting at block `first` of the operand's stages at LDS address `lds`.
 template <int R, int B, bool kSlow>
 struct Fragments {
-  static constexpr int kReads = kSlow ? 2 : 1;      // LDS instructions per fragment
   unsigned addr[kSlow ? B : 2];
+  v2i lo[2][kSlow ? B : 1], hi[2][kSlow ? B : 1];     // of the two halves of a stage
+  v4i whole[2][kSlow ? 1 : B];
 
   __device__ void init(unsigned lds, int first) {
     const int lane = threadIdx.x & 63;
@@ -119,33 +125,40 @@ struct Fragments {
     if constexpr (kSlow) {
       const int t = ((i >> 2) | ((g & 1) << 2)) & (R / 16 - 1);      // Source::turn of steps 8 g + i / 4 (+ 4, + 32)
 #pragma unroll
-      for (int b = 0; b < B; ++b)
-        addr[b] = lds + (8 * g + (i >> 2)) * (2 * R) + (((first + b) ^ t) << 5) + (i & 3) * 8;
+      for (int b = 0; b < B; ++b) addr[b] = lds + (8 * g + (i >> 2)) * (2 * R) + (((first + b) ^ t) << 5) + (i & 3) * 8;
     } else {
       addr[0] = lds + (first * 16 + i) * kStageBytes + ((g ^ (i >> 1)) << 4);
       addr[1] = addr[0] ^ 64;
     }
   }
-  // block b, half `sub` of the stage in buffer `buf`
-  template <int BUF, int SUB, int BLK>
-  __device__ void read(v2i& lo, v2i& hi, v4i& whole) const {
+  __device__ void other_buffer(int step) {
+#pragma unroll
+    for (int b = 0; b < (kSlow ? B : 2); ++b) addr[b] += step;
+  }
+  template <int SUB, int BLK>
+  __device__ void read() {
     if constexpr (kSlow) {
-      lo = lds_read_tr16<BUF * R * kStageBytes + SUB * 64 * R>(addr[BLK]);
-      hi = lds_read_tr16<BUF * R * kStageBytes + SUB * 64 * R + 8 * R>(addr[BLK]);
+      lo[SUB][BLK] = lds_read_tr16<SUB * 64 * R>(addr[BLK]);
+      hi[SUB][BLK] = lds_read_tr16<SUB * 64 * R + 8 * R>(addr[BLK]);
     } else {
-      whole = lds_read_b128_at<BUF * R * kStageBytes + BLK * 16 * kStageBytes>(addr[SUB]);
+      whole[SUB][BLK] = lds_read_b128_at<BLK * 16 * kStageBytes>(addr[SUB]);
     }
   }
-};
-
-template <bool kSlow>
-struct Frag {
-  v2i lo, hi;
-  v4i whole;
-  __device__ v4i landed() {
-    if constexpr (kSlow) return lds_landed(lo, hi);
-    asm volatile("" : "+v"(whole));
-    return whole;
+  // behind a settle: the reads of half SUB are in their registers
+  template <int SUB>
+  __device__ void landed() {
+    if constexpr (kSlow) {
+#pragma unroll
+      for (int b = 0; b < B; ++b) asm volatile("" : "+v"(lo[SUB][b]), "+v"(hi[SUB][b]));
+    } else {
+#pragma unroll
+      for (int b = 0; b < B; ++b) asm volatile("" : "+v"(whole[SUB][b]));
+    }
+  }
+  template <int SUB, int BLK>
+  __device__ v4i get() const {
+    if constexpr (kSlow) return v4i{lo[SUB][BLK][0], lo[SUB][BLK][1], hi[SUB][BLK][0], hi[SUB][BLK][1]};
+    else return whole[SUB][BLK];
   }
 };
 
@@ -154,6 +167,9 @@ __device__ inline v4f multiply(v4i a, v4i b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
+// Main loop.  Half a stage's fragments are read while the other half is multiplied, and the barrier lies between the halves: behind it
+// the next stage's first half is requested in front of the second half's products, and the loads of the stage after that go out, so no
+// product waits for the reads behind a barrier.  The fragments carried into the next turn have landed by the end of one.
 template <class T, bool kXSlow, bool kYSlow, class Acc>
 struct Product {
   Source<T::TI, kXSlow, T::kWaves> sx;
@@ -163,32 +179,48 @@ struct Product {
   Acc acc[T::BI][T::BJ];
   unsigned ldsx, ldsy;
 
+  static constexpr int kLoadsX = decltype(sx)::kLoads, kLoadsY = decltype(sy)::kLoads;
+
+  // instruction q of a stage's loads into buffer buf
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rx, __amdgpu_buffer_rsrc_t ry, int buf, int q) const {
+    if (q < kLoadsX) sx.load(rx, ldsx + buf * T::TI * kStageBytes, q);
+    else sy.load(ry, ldsy + buf * T::TJ * kStageBytes, q - kLoadsX);
+  }
   __device__ void issue(int buf) {
-    sx.issue(ldsx + buf * T::TI * kStageBytes);
-    sy.issue(ldsy + buf * T::TJ * kStageBytes);
+    const __amdgpu_buffer_rsrc_t rx = sx.stage(), ry = sy.stage();
+    static_for<kLoadsX + kLoadsY>([&](auto q) { load(rx, ry, buf, decltype(q)::value); });
+    sx.next();
+    sy.next();
   }
-
-  template <int BUF>
-  __device__ void stage() {
-    static_for<2>([&](auto sub) {
-      constexpr int SUB = decltype(sub)::value;
-      Frag<kXSlow> x[T::BI];
-      Frag<kYSlow> y[T::BJ];
-      static_for<T::BJ>([&](auto j) { fy.template read<BUF, SUB, decltype(j)::value>(y[j].lo, y[j].hi, y[j].whole); });
-      static_for<T::BI>([&](auto i) { fx.template read<BUF, SUB, decltype(i)::value>(x[i].lo, x[i].hi, x[i].whole); });
-      v4i yv[T::BJ];
-      static_for<T::BI>([&](auto i) {
-        constexpr int I = decltype(i)::value;
-        constexpr int kBehind = (T::BI - 1 - I) * Fragments<T::TI, T::BI, kXSlow>::kReads;
-        lds_settle<(kBehind < 15 ? kBehind : 15)>();
-        if constexpr (I == 0) static_for<T::BJ>([&](auto j) { yv[j] = y[j].landed(); });
-        const v4i xv = x[I].landed();
-        static_for<T::BJ>([&](auto j) { acc[I][j] = multiply(xv, yv[j], acc[I][j]); });
+  // Products of half SUB; half NEXT is read in between, and where kLoad the next stage but one goes out into buffer buf, spread over the
+  // products: a unit's loads pass at 64 bytes a clock, and a wavefront waits at a load that finds the queue full
+  template <int SUB, int NEXT, bool kLoad>
+  __device__ void half(int buf) {
+    const __amdgpu_buffer_rsrc_t rx = sx.stage(), ry = sy.stage();
+    static_for<T::BI>([&](auto i) {
+      constexpr int I = decltype(i)::value;
+      if constexpr (I < T::BJ) fy.template read<NEXT, I>();
+      fx.template read<NEXT, I>();
+     __builtin_amdgcn_s_setprio(1);  static_for<T::BJ>([&](auto j) {
+        constexpr int J = decltype(j)::value;
+        acc[I][J] = multiply(fx.template get<SUB, I>(), fy.template get<SUB, J>(), acc[I][J]);
       });
+      if constexpr (kLoad) {
+        constexpr int kAll = kLoadsX + kLoadsY, kFrom = I * kAll / T::BI, kTo = (I + 1) * kAll / T::BI;
+        static_for<kTo - kFrom>([&](auto q) { load(rx, ry, buf, kFrom + decltype(q)::value); });
+      }
+    __builtin_amdgcn_s_setprio(0);  __builtin_amdgcn_sched_barrier(0);      // keeps reads, products and loads in this order
     });
+    if constexpr (kLoad) {
+      sx.next();
+      sy.next();
+    }
+    lds_settle<0>();
+    fx.template landed<NEXT>();
+    fy.template landed<NEXT>();
   }
 
-  // x, y: operands; i0, j0: the tile's corner; range of the reduction: stages k0 .. k0 + n, ending at k_end (bytes or steps)
+  // x, y: operands; i0, j0: the tile's corner; range of the reduction: stages k0 .. k0 + n, ending at x_end and y_end (bytes or steps)
   __device__ void run(const VocabOperand& x, const VocabOperand& y, int i0, int j0, int k0, int n, int x_end, int y_end, char* smem) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     ldsx = lds_addr(smem);
@@ -201,19 +233,27 @@ struct Product {
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
       for (int j = 0; j < T::BJ; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+    // loads of the two stages behind the last are issued like the others: they are out of range, and what they clear is not multiplied
     issue(0);
-    int s = 0;
-    for (; s + 2 <= n; s += 2) {
-      tile_sync();          // the stage has landed, and the other buffer has been read by every wavefront
-      issue(1);
-      stage<0>();
-      tile_sync();
-      if (s + 2 < n) issue(0);
-      stage<1>();
-    }
-    if (s < n) {
-      tile_sync();
-      stage<0>();
+    issue(1);
+    constexpr int kLeast = (Source<T::TI, kXSlow, T::kWaves>::kInstructions + Source<T::TJ, kYSlow, T::kWaves>::kInstructions) / T::kWaves;   // loads per stage
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeast) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    static_for<T::BJ>([&](auto j) { fy.template read<0, decltype(j)::value>(); });
+    static_for<T::BI>([&](auto i) { fx.template read<0, decltype(i)::value>(); });
+    lds_settle<0>();
+    fx.template landed<0>();
+    fy.template landed<0>();
+    int buf = 0;
+    for (int s = 0; s < n; ++s) {
+      half<0, 1, false>(buf);
+      tile_sync();          // the next stage has landed, and this one's buffer has been read by every wavefront
+      const int step = buf == 0 ? 1 : -1;
+      fx.other_buffer(step * T::TI * kStageBytes);
+      fy.other_buffer(step * T::TJ * kStageBytes);
+      half<1, 0, true>(buf);
+      buf ^= 1;
     }
     tile_sync();            // the buffers are free
   }
@@ -239,7 +279,7 @@ __device__ inline float exp2_scale(const VocabLogits& l) {
 }
 
 template <class T>
-__global__ __launch_bounds__(T::kThreads) void vocab_stats_kernel(const VocabLogits l, const VocabStats st) {
+__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(const VocabLogits l, const VocabStats st) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int bi, bj;
   tile_of(blockIdx.x, (l.classes + T::TI - 1) / T::TI, (l.rows + T::TJ - 1) / T::TJ, &bi, &bj);
@@ -293,7 +333,7 @@ __global__ __launch_bounds__(T::kThreads) void vocab_stats_kernel(const VocabLog
 }
 
 template <class T>
-__global__ __launch_bounds__(T::kThreads) void vocab_grad_kernel(const VocabLogits l, const VocabGrad g) {
+__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(const VocabLogits l, const VocabGrad g) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   int bi, bj;
   tile_of(blockIdx.x, (l.classes + T::TI - 1) / T::TI, (l.rows + T::TJ - 1) / T::TJ, &bi, &bj);
@@ -340,7 +380,7 @@ __device__ inline int sums_exponent(const VocabSums& s) { return *s.exponent + s
 __device__ inline float sums_weight(const VocabSums& s, int j) { return s.weight == nullptr ? s.t : s.t * s.weight[s.weight_n == 1 ? 0 : j]; }
 
 template <class T, bool kYSlow>
-__global__ __launch_bounds__(T::kThreads) void vocab_sums_kernel(const VocabSums s) {
+__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_sums_kernel(const VocabSums s) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int ti = (s.ni + T::TI - 1) / T::TI, tj = (s.nj + T::TJ - 1) / T::TJ;
   const int slice = blockIdx.x / (ti * tj);
