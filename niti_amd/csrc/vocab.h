@@ -11,16 +11,16 @@
 
 namespace niti {
 
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 // p and g lie in [-1, 1]; as 16-bit floats they are kept times 2^15: eleven significant bits down to 2^-29, where bfloat16 has eight
 constexpr int kGradExponent = 15;
-// rows of the second product's left operand: activation times row weight over the largest row weight's power of two, times 2^8
+// rows of the weight gradient's left operand: activation times row weight over the power of two above the largest row weight, times 2^8
 constexpr int kRowExponent = 8;
 constexpr int kVocabTopMost = 1024;      // places of a teacher's list (one row's are kept in LDS)
-constexpr int kVocabClassTile = 256;     // classes that leave one (maximum, sum) pair of a row
 
 // What a forward pass leaves of a row: m, L (float), the sum of the targets' weights (float: 1; 0, nothing to learn from; NaN,
 // undefined), a word of nothing, then for each of its `top` places g / T (float) and the class, -1 where there is none or an earlier place
@@ -29,7 +29,7 @@ inline __host__ __device__ long long vocab_state_words(int top) { return 4 + (2L
 
 // One operand of a product tile: rows of `pitch` bytes, 16-byte aligned.
 //   reduction index fast: `rows` rows of `row_bytes` bytes (a multiple of 16)
-//   reduction index slow: `rows` steps of the reduction, tile columns along the row
+//   reduction index slow: `rows` steps of the reduction, tile columns along the row, whose readable length is row_bytes
 struct VocabOperand {
   const void* p;
   long long pitch;
@@ -45,16 +45,32 @@ struct VocabLogits {         // s[v][n] = w[v] . a[n]
   float inv_t;               // 1 / T
 };
 
-struct VocabStats {          // (max, sum of 2^((s - max) k)) of each row over each kVocabClassTile classes
+struct VocabStats {          // (max, sum of 2^((s - max) k)) of each row over each tile's classes
   int2* part;                // [rows][tiles]
   int tiles;
+};
+
+// int8 rows to 16-bit floats, each times weight / 2^*exponent 2^kRowExponent where there are weights; *exponent receives the smallest power of
+// two above every weight
+struct VocabWiden {
+  const int8_t* src;         // 16-byte aligned rows, zero up to the next multiple of 16 values
+  long long src_pitch;
+  _Float16* dst;
+  long long pitch;
+  int rows, values;
+  const float* weight;
+  int32_t* exponent;
+  int blocks;                // 0: nothing to do
 };
 
 struct VocabGrad {           // sum_j q_j p, times 2^kGradExponent, of the classes of a piece
   const int32_t* state;      // [rows][state_words]
   long long state_words;
+  int top;                   // targets written into the piece here; 0: vocab_targets_kernel does it
+  long long first;           // class that the piece starts at
   _Float16* g;               // [rows][pitch], zero between the piece's last class and the next multiple of eight
   long long pitch;
+  VocabWiden widen;          // done by workgroups of its own
 };
 
 struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
@@ -74,10 +90,16 @@ struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
   int weight_n;
 };
 
-int launch_vocab_stats(const VocabLogits& l, const VocabStats& s, hipStream_t stream);
-int launch_vocab_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream);
-int launch_vocab_sums(const VocabSums& s, bool y_slow, hipStream_t stream);   // x's reduction index is the slow one, y's may be
-int launch_vocab_join(const VocabSums& s, hipStream_t stream);
-void vocab_sums_plan(int ni, int nj, int nk, int* slices, int* steps);
+enum VocabTile { kVocabLarge, kVocabMiddle, kVocabFew };
+VocabTile vocab_logits_tile(int rows, int classes);
+int vocab_stats_tiles(VocabTile t, int classes);    // pairs that launch_vocab_stats leaves of a row
+bool vocab_grad_writes_targets(VocabTile t, int top);
+int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream);
+int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hipStream_t stream);
+// Both gradients' sums of a piece: a = the activations' (x: int8 weights, reduction slow; y: the piece's gradient, reduction fast), w = the
+// weights' (x: 16-bit activations, y: the piece's gradient, reduction slow in both)
+VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w);
+int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream);
+int launch_vocab_join(const VocabSums* a, const VocabSums* w, hipStream_t stream);   // either may be null
 
 }  // namespace niti

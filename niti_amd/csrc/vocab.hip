@@ -2,11 +2,17 @@
 // two gradients behind it.  One tile product serves all three.
 //
 // Tile: TI x TJ results of sum_k x[i][k] y[j][k]; lane l of a wavefront holds for each 16 x 16 block column j = l % 16 and the rows
-// i = 4 (l / 16) .. + 4 (v_mfma_i32_16x16x64_i8 or v_mfma_f32_16x16x32_f16, 64 bytes of the reduction each).  A stage is 128 bytes of
-// the reduction, two buffers, filled by buffer_load ... lds while the other one is multiplied.  An operand whose reduction
-// index is fast is staged as whole 128-byte lines, 16-byte pieces XOR-swizzled by row / 2 so that the 16 rows a fragment read takes lie in
-// different banks; one whose reduction index is slow (16-bit values only) lies as stored, 64 steps of TI or TJ columns, and is
-// transposed by ds_read_b64_tr_b16, its 32-byte pieces XOR-swizzled by the step.
+// i = 4 (l / 16) .. + 4 (v_mfma_i32_16x16x64_i8 or v_mfma_f32_16x16x32_f16).  A stage is 128 bytes of an int8 reduction, 64 steps of a
+// 16-bit one, in two buffers, filled by buffer_load ... lds while the other one is multiplied.  An operand lies in a stage
+//   kFast    as whole 128-byte lines of its rows, 16-byte pieces XOR-swizzled by row / 2 so that the 16 rows a fragment read takes lie
+//            in different banks
+//   kSlow16  as stored with a slow reduction index, 64 steps of 16-bit columns, transposed by ds_read_b64_tr_b16, its 32-byte pieces
+//            XOR-swizzled by the step
+//   kSlow8   the same of int8 columns, transposed by ds_read_b64_tr_b8 and made 16-bit floats in registers (exact)
+//
+// What bounds the large tile (8192 x 8192 x 4096, 512 tiles, 2.1 GHz): a stage's products alone take 2048 clocks, its loads pass at 64
+// bytes a clock (64 KB: 1024), its fragments are 192 KB of LDS reads.  Gradient sums 393 - 423 us; with the loads left out 360 - 380, with
+// products alone 307 - 335; loads issued all at once behind the barrier 425 - 464.
 #include "lds_asm.h"
 #include "vocab.h"
 
@@ -14,7 +20,11 @@ namespace niti {
 namespace {
 
 constexpr int kFar = static_cast<int>(0x80000000u);   // beyond every buffer: reads as zero
-constexpr int kStageBytes = 128;                      // of the reduction
+constexpr int kStageBytes = 128;                      // of a fast reduction
+constexpr int kNone = -2147483647 - 1;                // below every logit
+
+enum Layout { kFast, kSlow16, kSlow8 };
+constexpr int stage_bytes(int r, Layout l) { return l == kSlow8 ? 64 * r : kStageBytes * r; }
 
 template <int TI_, int TJ_, int WI_, int WJ_>
 struct Tile {
@@ -27,7 +37,7 @@ struct Tile {
 };
 typedef Tile<256, 256, 2, 4> TileLarge;
 typedef Tile<128, 128, 2, 2> TileMiddle;
-typedef Tile<256, 32, 8, 1> TileFew;
+typedef Tile<128, 32, 4, 1> TileFew;
 
 // 16-lane groups: lane i of a group names 8 bytes of a 4 x 16 block of 16-bit values (row i / 4, columns 4 (i % 4) .. + 4) and receives
 // column i of it
@@ -44,12 +54,28 @@ __device__ inline void tile_sync() {
   asm volatile("" ::: "memory");
 }
 
-// One operand's way from memory to fragments: R rows (or columns, where the reduction index is slow).
-template <int R, bool kSlow, int kWaves>
+// eight int8 values as 16-bit floats, exactly: a byte b + 128 under the exponent of 1024 is 1024 + 128 + b
+__device__ inline v4i widen8(v2i b) {
+  const v2h bias = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+  v4i o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const unsigned u = static_cast<unsigned>(b[h]) ^ 0x80808080u;
+    const unsigned lo = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u), hi = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
+    o[2 * h] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, lo) + bias);
+    o[2 * h + 1] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, hi) + bias);
+  }
+  return o;
+}
+
+// One operand's way from memory to its stages: R rows (or columns, where the reduction index is slow).
+template <int R, Layout L, int kWaves>
 struct Source {
-  static constexpr int kInstructions = R * kStageBytes / 1024;              // of a stage
+  static constexpr bool kSlow = L != kFast;
+  static constexpr int kStage = stage_bytes(R, L);
+  static constexpr int kInstructions = kStage / 1024;                       // of a stage
   static constexpr int kLoads = (kInstructions + kWaves - 1) / kWaves;      // of a wavefront, 16 bytes per lane each
-  static constexpr int kRowBytes = kSlow ? 2 * R : kStageBytes;
+  static constexpr int kRowBytes = L == kFast ? kStageBytes : (L == kSlow16 ? 2 * R : R);
   static constexpr int kRowsPerLoad = 1024 / kRowBytes;
   static constexpr int kPieces = kRowBytes / 16;
   static_assert(kInstructions % kWaves == 0 || kInstructions < kWaves, "whole wavefronts");
@@ -57,24 +83,23 @@ struct Source {
   const char* base;
   long long left;        // bytes from base to the end of the matrix
   long long advance;     // per stage
-  int fast_left;         // bytes of the reduction left in a row (reduction fast)
+  int fast_left;         // bytes of the reduction left in a row (kFast)
   int voff[kLoads];
   int piece;
 
-  // slow position of a reduction step within its stage that its 32-byte pieces are swizzled by: the eight steps that 32 lanes read
-  // at once (four of each 16-lane group, groups eight steps apart) differ in it
-  static __device__ int turn(int k) { return ((k & 3) | (((k >> 3) & 1) << 2)) & (R / 16 - 1); }
+  // what a step's pieces are swizzled by: the steps that 32 lanes read at once differ in it (kSlow16: four of each 16-lane group, groups
+  // eight steps apart; kSlow8: eight of each)
+  static __device__ int turn(int k) { return (L == kSlow16 ? (k & 3) | (((k >> 3) & 1) << 2) : k & 15) & (R / 16 - 1); }
 
-  // first: first row (fast) or column (slow) of the tile; k0: first reduction step in stages; k_end: end of the reduction's range in bytes (fast)
-  // or steps (slow)
+  // first: first row (fast) or column (slow) of the tile; k0: first stage; k_end: end of the reduction's range in bytes (fast) or steps (slow)
   __device__ void init(const VocabOperand& o, int first, int k0, int k_end) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const char* const p = static_cast<const char*>(o.p);
     if (kSlow) {
-      const long long skip = static_cast<long long>(k0) * 64 * o.pitch + 2LL * first;
+      const long long skip = static_cast<long long>(k0) * 64 * o.pitch + (L == kSlow16 ? 2LL : 1LL) * first;
       base = p + skip;
-      left = static_cast<long long>(k_end) * o.pitch - skip;
+      left = (k_end - 1) * o.pitch + o.row_bytes - skip;
       advance = 64 * o.pitch;
       fast_left = 0;
       piece = 0;
@@ -89,7 +114,7 @@ struct Source {
     for (int q = 0; q < kLoads; ++q) {
       const int row = (q * kWaves + wave) * kRowsPerLoad + lane / kPieces;
       const int slot = lane % kPieces;
-      const int c = kSlow ? slot ^ (2 * turn(row)) : slot ^ ((row >> 1) & 7);
+      const int c = L == kFast ? slot ^ ((row >> 1) & 7) : (L == kSlow16 ? slot ^ (2 * turn(row)) : slot ^ turn(row));
       if (!kSlow) piece = c * 16;       // the same for every q: a load's rows are a multiple of 16 apart
       voff[q] = static_cast<int>(row * o.pitch) + c * 16;
     }
@@ -112,34 +137,39 @@ struct Source {
   }
 };
 
-// Fragment reads of B blocks of 16 rows / columns, starting at block `first` of the operand's stages at LDS address `lds`.
-template <int R, int B, bool kSlow>
+// Fragments of B blocks of 16 rows / columns, starting at block `first` of the operand's stages at LDS address `lds`.
+template <int R, int B, Layout L>
 struct Fragments {
-  unsigned addr[kSlow ? B : 2];
-  v2i lo[2][kSlow ? B : 1], hi[2][kSlow ? B : 1];     // of the two halves of a stage
-  v4i whole[2][kSlow ? 1 : B];
+  static constexpr int kAddr = L == kFast ? 2 : B;
+  unsigned addr[kAddr];
+  v2i lo[2][L == kFast ? 1 : B], hi[2][L == kSlow16 ? B : 1];     // of the two halves of a stage
+  v4i whole[2][L == kFast ? B : 1];
 
   __device__ void init(unsigned lds, int first) {
     const int lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
-    if constexpr (kSlow) {
-      const int t = ((i >> 2) | ((g & 1) << 2)) & (R / 16 - 1);      // Source::turn of steps 8 g + i / 4 (+ 4, + 32)
-#pragma unroll
-      for (int b = 0; b < B; ++b) addr[b] = lds + (8 * g + (i >> 2)) * (2 * R) + (((first + b) ^ t) << 5) + (i & 3) * 8;
-    } else {
+    if constexpr (L == kFast) {
       addr[0] = lds + (first * 16 + i) * kStageBytes + ((g ^ (i >> 1)) << 4);
       addr[1] = addr[0] ^ 64;
+    } else {
+      const int step = 8 * g + (L == kSlow16 ? i >> 2 : i >> 1);
+      const int t = Source<R, L, 1>::turn(step);     // the same for the other steps that this lane names
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+        addr[b] = L == kSlow16 ? lds + step * (2 * R) + (((first + b) ^ t) << 5) + (i & 3) * 8 : lds + step * R + (((first + b) ^ t) << 4) + (i & 1) * 8;
     }
   }
   __device__ void other_buffer(int step) {
 #pragma unroll
-    for (int b = 0; b < (kSlow ? B : 2); ++b) addr[b] += step;
+    for (int b = 0; b < kAddr; ++b) addr[b] += step;
   }
   template <int SUB, int BLK>
   __device__ void read() {
-    if constexpr (kSlow) {
+    if constexpr (L == kSlow16) {
       lo[SUB][BLK] = lds_read_tr16<SUB * 64 * R>(addr[BLK]);
       hi[SUB][BLK] = lds_read_tr16<SUB * 64 * R + 8 * R>(addr[BLK]);
+    } else if constexpr (L == kSlow8) {
+      lo[SUB][BLK] = lds_read_tr8<SUB * 32 * R>(addr[BLK]);
     } else {
       whole[SUB][BLK] = lds_read_b128_at<BLK * 16 * kStageBytes>(addr[SUB]);
     }
@@ -147,17 +177,17 @@ struct Fragments {
   // behind a settle: the reads of half SUB are in their registers
   template <int SUB>
   __device__ void landed() {
-    if constexpr (kSlow) {
 #pragma unroll
-      for (int b = 0; b < B; ++b) asm volatile("" : "+v"(lo[SUB][b]), "+v"(hi[SUB][b]));
-    } else {
-#pragma unroll
-      for (int b = 0; b < B; ++b) asm volatile("" : "+v"(whole[SUB][b]));
+    for (int b = 0; b < B; ++b) {
+      if constexpr (L == kSlow16) asm volatile("" : "+v"(lo[SUB][b]), "+v"(hi[SUB][b]));
+      else if constexpr (L == kSlow8) asm volatile("" : "+v"(lo[SUB][b]));
+      else asm volatile("" : "+v"(whole[SUB][b]));
     }
   }
   template <int SUB, int BLK>
   __device__ v4i get() const {
-    if constexpr (kSlow) return v4i{lo[SUB][BLK][0], lo[SUB][BLK][1], hi[SUB][BLK][0], hi[SUB][BLK][1]};
+    if constexpr (L == kSlow16) return v4i{lo[SUB][BLK][0], lo[SUB][BLK][1], hi[SUB][BLK][0], hi[SUB][BLK][1]};
+    else if constexpr (L == kSlow8) return widen8(lo[SUB][BLK]);
     else return whole[SUB][BLK];
   }
 };
@@ -168,23 +198,24 @@ __device__ inline v4f multiply(v4i a, v4i b, v4f c) {
 }
 
 // Main loop.  Half a stage's fragments are read while the other half is multiplied, and the barrier lies between the halves: behind it
-// the next stage's first half is requested in front of the second half's products, and the loads of the stage after that go out, so no
+// the next stage's first half is requested along with the second half's products, and the loads of the stage after that go out, so no
 // product waits for the reads behind a barrier.  The fragments carried into the next turn have landed by the end of one.
-template <class T, bool kXSlow, bool kYSlow, class Acc>
+template <class T, Layout LX, Layout LY, class Acc>
 struct Product {
-  Source<T::TI, kXSlow, T::kWaves> sx;
-  Source<T::TJ, kYSlow, T::kWaves> sy;
-  Fragments<T::TI, T::BI, kXSlow> fx;
-  Fragments<T::TJ, T::BJ, kYSlow> fy;
+  Source<T::TI, LX, T::kWaves> sx;
+  Source<T::TJ, LY, T::kWaves> sy;
+  Fragments<T::TI, T::BI, LX> fx;
+  Fragments<T::TJ, T::BJ, LY> fy;
   Acc acc[T::BI][T::BJ];
   unsigned ldsx, ldsy;
-
-  static constexpr int kLoadsX = decltype(sx)::kLoads, kLoadsY = decltype(sy)::kLoads;
+  static constexpr int kStageX = stage_bytes(T::TI, LX), kStageY = stage_bytes(T::TJ, LY);
+  static constexpr int kLoadsX = Source<T::TI, LX, T::kWaves>::kLoads, kLoadsY = Source<T::TJ, LY, T::kWaves>::kLoads;
+  static_assert(2 * (kStageX + kStageY) <= T::kLds, "stages fit");
 
   // instruction q of a stage's loads into buffer buf
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rx, __amdgpu_buffer_rsrc_t ry, int buf, int q) const {
-    if (q < kLoadsX) sx.load(rx, ldsx + buf * T::TI * kStageBytes, q);
-    else sy.load(ry, ldsy + buf * T::TJ * kStageBytes, q - kLoadsX);
+    if (q < kLoadsX) sx.load(rx, ldsx + buf * kStageX, q);
+    else sy.load(ry, ldsy + buf * kStageY, q - kLoadsX);
   }
   __device__ void issue(int buf) {
     const __amdgpu_buffer_rsrc_t rx = sx.stage(), ry = sy.stage();
@@ -197,19 +228,23 @@ struct Product {
   template <int SUB, int NEXT, bool kLoad>
   __device__ void half(int buf) {
     const __amdgpu_buffer_rsrc_t rx = sx.stage(), ry = sy.stage();
+    static_for<(T::BJ > T::BI ? T::BJ - T::BI : 0)>([&](auto j) { fy.template read<NEXT, T::BI + decltype(j)::value>(); });
     static_for<T::BI>([&](auto i) {
       constexpr int I = decltype(i)::value;
       if constexpr (I < T::BJ) fy.template read<NEXT, I>();
       fx.template read<NEXT, I>();
-     __builtin_amdgcn_s_setprio(1);  static_for<T::BJ>([&](auto j) {
+      __builtin_amdgcn_s_setprio(1);
+      const v4i x = fx.template get<SUB, I>();
+      static_for<T::BJ>([&](auto j) {
         constexpr int J = decltype(j)::value;
-        acc[I][J] = multiply(fx.template get<SUB, I>(), fy.template get<SUB, J>(), acc[I][J]);
+        acc[I][J] = multiply(x, fy.template get<SUB, J>(), acc[I][J]);
       });
+      __builtin_amdgcn_s_setprio(0);
       if constexpr (kLoad) {
         constexpr int kAll = kLoadsX + kLoadsY, kFrom = I * kAll / T::BI, kTo = (I + 1) * kAll / T::BI;
         static_for<kTo - kFrom>([&](auto q) { load(rx, ry, buf, kFrom + decltype(q)::value); });
       }
-    __builtin_amdgcn_s_setprio(0);  __builtin_amdgcn_sched_barrier(0);      // keeps reads, products and loads in this order
+      __builtin_amdgcn_sched_barrier(0);      // reads, products and loads stay in this order
     });
     if constexpr (kLoad) {
       sx.next();
@@ -224,7 +259,7 @@ struct Product {
   __device__ void run(const VocabOperand& x, const VocabOperand& y, int i0, int j0, int k0, int n, int x_end, int y_end, char* smem) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     ldsx = lds_addr(smem);
-    ldsy = ldsx + 2 * T::TI * kStageBytes;
+    ldsy = ldsx + 2 * kStageX;
     sx.init(x, i0, k0, x_end);
     sy.init(y, j0, k0, y_end);
     fx.init(ldsx, (wave / T::WJ) * T::BI);
@@ -236,7 +271,7 @@ struct Product {
     // loads of the two stages behind the last are issued like the others: they are out of range, and what they clear is not multiplied
     issue(0);
     issue(1);
-    constexpr int kLeast = (Source<T::TI, kXSlow, T::kWaves>::kInstructions + Source<T::TJ, kYSlow, T::kWaves>::kInstructions) / T::kWaves;   // loads per stage
+    constexpr int kLeast = Source<T::TI, LX, T::kWaves>::kInstructions / T::kWaves + Source<T::TJ, LY, T::kWaves>::kInstructions / T::kWaves;   // per stage
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeast) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -250,8 +285,8 @@ struct Product {
       half<0, 1, false>(buf);
       tile_sync();          // the next stage has landed, and this one's buffer has been read by every wavefront
       const int step = buf == 0 ? 1 : -1;
-      fx.other_buffer(step * T::TI * kStageBytes);
-      fy.other_buffer(step * T::TJ * kStageBytes);
+      fx.other_buffer(step * kStageX);
+      fy.other_buffer(step * kStageY);
       half<1, 0, true>(buf);
       buf ^= 1;
     }
@@ -284,7 +319,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
   int bi, bj;
   tile_of(blockIdx.x, (l.classes + T::TI - 1) / T::TI, (l.rows + T::TJ - 1) / T::TJ, &bi, &bj);
   const int i0 = bi * T::TI, j0 = bj * T::TJ;
-  Product<T, false, false, v4i> p;
+  Product<T, kFast, kFast, v4i> p;
   p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -295,7 +330,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
   const bool whole = i0 + T::TI <= l.classes;
 #pragma unroll
   for (int j = 0; j < T::BJ; ++j) {
-    int m = -2147483647 - 1;
+    int m = kNone;
 #pragma unroll
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
@@ -314,9 +349,6 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
     if (lane < 16) park[wi * T::TJ + (wj * T::BJ + j) * 16 + lane] = make_int2(m, __float_as_int(sum));
   }
   __syncthreads();
-  // one pair of each row for every kVocabClassTile classes
-  constexpr int kGroups = T::TI < kVocabClassTile ? 1 : T::TI / kVocabClassTile;
-  static_assert(kGroups == 1, "a tile leaves one pair");
   for (int j = threadIdx.x; j < T::TJ; j += T::kThreads) {
     if (j0 + j >= l.rows) break;
     int m = park[j].x;
@@ -326,47 +358,110 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
 #pragma unroll
     for (int i = 0; i < T::WI; ++i) {
       const int2 v = park[i * T::TJ + j];
-      if (v.x != -2147483647 - 1) sum += __int_as_float(v.y) * __builtin_amdgcn_exp2f(static_cast<float>(v.x - m) * k);
+      if (v.x != kNone) sum += __int_as_float(v.y) * __builtin_amdgcn_exp2f(static_cast<float>(v.x - m) * k);
     }
     st.part[static_cast<long long>(j0 + j) * st.tiles + bi] = make_int2(m, __float_as_int(sum));
   }
 }
 
+__device__ inline void widen_block(const VocabWiden& w, int block, int threads, char* smem) {
+  float scale = 1.0f;
+  int e = 0;
+  if (w.weight != nullptr) {
+    float* const most = reinterpret_cast<float*>(smem);
+    float m = 0.0f;
+    for (int i = threadIdx.x; i < w.rows; i += threads) m = fmaxf(m, fabsf(w.weight[i]));
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+    __syncthreads();
+    for (int i = 0; i < threads / 64; ++i) m = fmaxf(m, most[i]);
+    if (m > 0.0f) frexpf(fminf(m, 3.402823466e38f), &e);
+    if (block == 0 && threadIdx.x == 0) *w.exponent = e;
+  }
+  const int pieces = (w.values + 15) / 16;
+  const long long all = static_cast<long long>(w.rows) * pieces;
+  for (long long at = static_cast<long long>(block) * threads + threadIdx.x; at < all; at += static_cast<long long>(w.blocks) * threads) {
+    const long long row = at / pieces;
+    const int c = static_cast<int>(at - row * pieces) * 16;
+    union {
+      int8_t b[16];
+      v4i v;
+    } u;
+    u.v = *reinterpret_cast<const v4i*>(w.src + row * w.src_pitch + c);
+    if (w.weight != nullptr) scale = ldexpf(w.weight[row], kRowExponent - e);
+    v8h o[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i >> 3][i & 7] = static_cast<_Float16>(static_cast<float>(u.b[i]) * scale);
+    v8h* const out = reinterpret_cast<v8h*>(w.dst + row * w.pitch + c);
+    out[0] = o[0];
+    out[1] = o[1];
+  }
+}
+
+// A tile of 16-bit values on its way out: [TJ][TI], 16-byte pieces XOR-swizzled by the row, so that lanes that hold four neighbours of
+// 16 different rows write to different banks and rows leave as whole lines.
+template <class T>
+struct Outgoing {
+  static constexpr int kPieces = T::TI / 8;
+  char* smem;
+  __device__ char* at(int j, int piece) const { return smem + j * (2 * T::TI) + ((piece ^ (j & (kPieces - 1))) << 4); }
+  __device__ void put(int j, int i, uint64_t four) const { *reinterpret_cast<uint64_t*>(at(j, i >> 3) + ((i & 4) << 1)) = four; }
+  __device__ uint16_t* one(int j, int i) const { return reinterpret_cast<uint16_t*>(at(j, i >> 3)) + (i & 7); }
+};
+
 template <class T>
 __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(const VocabLogits l, const VocabGrad g) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
+  if (static_cast<int>(blockIdx.x) >= ti * tj) {
+    widen_block(g.widen, blockIdx.x - ti * tj, T::kThreads, smem);
+    return;
+  }
   int bi, bj;
-  tile_of(blockIdx.x, (l.classes + T::TI - 1) / T::TI, (l.rows + T::TJ - 1) / T::TJ, &bi, &bj);
+  tile_of(blockIdx.x, ti, tj, &bi, &bj);
   const int i0 = bi * T::TI, j0 = bj * T::TJ;
-  Product<T, false, false, v4i> p;
+  Product<T, kFast, kFast, v4i> p;
   p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / T::WJ, wj = wave % T::WJ;
   const float k = exp2_scale(l);
-  const int v0 = i0 + wi * T::BI * 16 + 4 * (lane >> 4);
-  const int padded = (l.classes + 7) & ~7;
+  const Outgoing<T> out{smem};
 #pragma unroll
   for (int j = 0; j < T::BJ; ++j) {
-    const int n = j0 + (wj * T::BJ + j) * 16 + (lane & 15);
-    if (n >= l.rows) continue;
-    const int32_t* const row = g.state + n * g.state_words;
-    const int m = row[0];
+    const int jt = (wj * T::BJ + j) * 16 + (lane & 15);
+    const v4i row = j0 + jt < l.rows ? *reinterpret_cast<const v4i*>(g.state + (j0 + jt) * g.state_words) : v4i{0, 0, 0, 0};
     const float shift = static_cast<float>(kGradExponent) - __int_as_float(row[1]);
     const float coef = __int_as_float(row[2]);
-    _Float16* const out = g.g + n * g.pitch;
 #pragma unroll
     for (int i = 0; i < T::BI; ++i) {
-      const int v = v0 + i * 16;
-      if (v >= padded) continue;
+      const int it = (wi * T::BI + i) * 16 + 4 * (lane >> 4);
       v4h o;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(static_cast<float>(p.acc[i][j][r] - m), k, shift)) * coef;
-        o[r] = static_cast<_Float16>(v + r < l.classes ? e : 0.0f);
+        const float e = __builtin_amdgcn_exp2f(fmaf(static_cast<float>(p.acc[i][j][r] - row[0]), k, shift)) * coef;
+        o[r] = static_cast<_Float16>(i0 + it + r < l.classes ? e : 0.0f);
       }
-      *reinterpret_cast<v4h*>(out + v) = o;
+      out.put(jt, it, __builtin_bit_cast(uint64_t, o));
     }
+  }
+  __syncthreads();
+  if (g.top > 0) {
+    const int rows = min(T::TJ, l.rows - j0), places = rows * g.top;
+    for (int at = threadIdx.x; at < places; at += T::kThreads) {
+      const int j = at / g.top;
+      const int2 s = *reinterpret_cast<const int2*>(g.state + (j0 + j) * g.state_words + 4 + 2 * (at - j * g.top));
+      const long long i = s.y - g.first - i0;
+      if (s.y >= 0 && i >= 0 && i < T::TI && i0 + i < l.classes)
+        *out.one(j, static_cast<int>(i)) = __builtin_bit_cast(uint16_t, static_cast<_Float16>(ldexpf(__int_as_float(s.x), kGradExponent)));
+    }
+    __syncthreads();
+  }
+  const int padded = (l.classes + 7) & ~7;
+  for (int at = threadIdx.x; at < T::TJ * Outgoing<T>::kPieces; at += T::kThreads) {
+    const int j = at / Outgoing<T>::kPieces, c = at % Outgoing<T>::kPieces;
+    if (j0 + j < l.rows && i0 + 8 * c < padded) *reinterpret_cast<v4i*>(g.g + (j0 + j) * g.pitch + i0 + 8 * c) = *reinterpret_cast<const v4i*>(out.at(j, c));
   }
 }
 
@@ -379,60 +474,83 @@ __device__ inline uint16_t bf16_of(float f) {   // round to nearest, ties to eve
 __device__ inline int sums_exponent(const VocabSums& s) { return *s.exponent + s.bias + (s.exponent2 != nullptr ? *s.exponent2 : 0); }
 __device__ inline float sums_weight(const VocabSums& s, int j) { return s.weight == nullptr ? s.t : s.t * s.weight[s.weight_n == 1 ? 0 : j]; }
 
-template <class T, bool kYSlow>
-__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_sums_kernel(const VocabSums s) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
+template <class T, Layout LX, Layout LY>
+__device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
   const int ti = (s.ni + T::TI - 1) / T::TI, tj = (s.nj + T::TJ - 1) / T::TJ;
-  const int slice = blockIdx.x / (ti * tj);
+  const int slice = block / (ti * tj);
+  if (slice >= s.slices) return;
   int bi, bj;
-  tile_of(blockIdx.x - slice * ti * tj, ti, tj, &bi, &bj);
+  tile_of(block - slice * ti * tj, ti, tj, &bi, &bj);
   const int i0 = bi * T::TI, j0 = bj * T::TJ;
   const int stages = (s.nk + 63) / 64;
   const int k0 = slice * s.steps;
   const int n = min(s.steps, stages - k0);
   const int end = min(s.nk, (k0 + n) * 64);      // steps
-  Product<T, true, kYSlow, v4f> p;
-  p.run(s.x, s.y, i0, j0, k0, n, end, kYSlow ? end : 2 * ((end + 7) & ~7), smem);
+  Product<T, LX, LY, v4f> p;
+  p.run(s.x, s.y, i0, j0, k0, n, LX == kFast ? 2 * ((end + 7) & ~7) : end, LY == kFast ? 2 * ((end + 7) & ~7) : end, smem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / T::WJ, wj = wave % T::WJ;
-  const int iw = i0 + wi * T::BI * 16 + 4 * (lane >> 4);
-  const int e = sums_exponent(s);
+  if (s.part != nullptr) {
 #pragma unroll
-  for (int j = 0; j < T::BJ; ++j) {
-    const int jj = j0 + (wj * T::BJ + j) * 16 + (lane & 15);
-    if (jj >= s.nj) continue;
-    const float weight = s.part == nullptr ? sums_weight(s, jj) : 1.0f;
+    for (int j = 0; j < T::BJ; ++j) {
+      const int jj = j0 + (wj * T::BJ + j) * 16 + (lane & 15);
+      if (jj >= s.nj) continue;
+      float* const row = s.part + (static_cast<long long>(slice) * s.nj + jj) * s.part_pitch;
 #pragma unroll
-    for (int i = 0; i < T::BI; ++i) {
-      const int ii = iw + i * 16;
-      if (ii >= s.ni) continue;
-      v4f v = p.acc[i][j];
-      if (s.part != nullptr) {
-        v4f* const at = reinterpret_cast<v4f*>(s.part + (static_cast<long long>(slice) * s.nj + jj) * s.part_pitch + ii);
+      for (int i = 0; i < T::BI; ++i) {
+        const int ii = i0 + (wi * T::BI + i) * 16 + 4 * (lane >> 4);
+        if (ii >= s.ni) continue;
+        v4f* const at = reinterpret_cast<v4f*>(row + ii);
+        v4f v = p.acc[i][j];
         if (s.accumulate) v += *at;
         *at = v;
-      } else {
-        uint16_t* const at = s.out + static_cast<long long>(jj) * s.ni + ii;
-        uint16_t b[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) b[r] = bf16_of(ldexpf(v[r] * weight, e));
-        if ((s.ni & 3) == 0) {
-          *reinterpret_cast<uint64_t*>(at) = b[0] | static_cast<uint64_t>(b[1]) << 16 | static_cast<uint64_t>(b[2]) << 32 | static_cast<uint64_t>(b[3]) << 48;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (ii + r < s.ni) at[r] = b[r];
-        }
       }
+    }
+    return;
+  }
+  const int e = sums_exponent(s);
+  const Outgoing<T> out{smem};
+#pragma unroll
+  for (int j = 0; j < T::BJ; ++j) {
+    const int jt = (wj * T::BJ + j) * 16 + (lane & 15);
+    const float weight = j0 + jt < s.nj ? sums_weight(s, j0 + jt) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < T::BI; ++i) {
+      uint64_t four = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) four |= static_cast<uint64_t>(bf16_of(ldexpf(p.acc[i][j][r] * weight, e))) << (16 * r);
+      out.put(jt, (wi * T::BI + i) * 16 + 4 * (lane >> 4), four);
+    }
+  }
+  __syncthreads();
+  if ((s.ni & 7) == 0) {
+    for (int at = threadIdx.x; at < T::TJ * Outgoing<T>::kPieces; at += T::kThreads) {
+      const int j = at / Outgoing<T>::kPieces, c = at % Outgoing<T>::kPieces;
+      if (j0 + j < s.nj && i0 + 8 * c < s.ni)
+        *reinterpret_cast<v4i*>(s.out + static_cast<long long>(j0 + j) * s.ni + i0 + 8 * c) = *reinterpret_cast<const v4i*>(out.at(j, c));
+    }
+  } else {      // rows that start anywhere: a value per lane, neighbours in neighbouring lanes
+    for (int at = threadIdx.x; at < T::TJ * T::TI; at += T::kThreads) {
+      const int j = at / T::TI, i = at % T::TI;
+      if (j0 + j < s.nj && i0 + i < s.ni) s.out[static_cast<long long>(j0 + j) * s.ni + i0 + i] = *out.one(j, i);
     }
   }
 }
 
+// Both gradients' sums: the first `blocks_a` workgroups (a multiple of eight, see tile_of) the activations', the others the weights'.
+template <class TA, class TW>
+__global__ __launch_bounds__(TA::kThreads, TA::kPerUnit) void vocab_sums_kernel(const VocabSums a, const VocabSums w, int blocks_a) {
+  static_assert(TA::kThreads == TW::kThreads, "one launch");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  if (static_cast<int>(blockIdx.x) < blocks_a) sums_tile<TA, kSlow8, kFast>(a, blockIdx.x, smem);
+  else sums_tile<TW, kSlow16, kSlow16>(w, blockIdx.x - blocks_a, smem);
+}
+
 // adds the slices, scales, rounds; a lane takes four neighbours of a row
-__global__ __launch_bounds__(256) void vocab_join_kernel(const VocabSums s) {
+__device__ inline void join_block(const VocabSums& s, long long block) {
   const int quads = (s.ni + 3) / 4;
-  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const long long at = block * 256 + threadIdx.x;
   if (at >= static_cast<long long>(quads) * s.nj) return;
   const int j = static_cast<int>(at / quads), i = static_cast<int>(at - static_cast<long long>(j) * quads) * 4;
   v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -450,7 +568,20 @@ __global__ __launch_bounds__(256) void vocab_join_kernel(const VocabSums s) {
   const float weight = sums_weight(s, j);
   const int e = sums_exponent(s);
   uint16_t* const out = s.out + static_cast<long long>(j) * s.ni + i;
-  for (int r = 0; r < 4 && i + r < s.ni; ++r) out[r] = bf16_of(ldexpf(v[r] * weight, e));
+  uint16_t b[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) b[r] = bf16_of(ldexpf(v[r] * weight, e));
+  if ((s.ni & 3) == 0) {
+    *reinterpret_cast<uint64_t*>(out) = b[0] | static_cast<uint64_t>(b[1]) << 16 | static_cast<uint64_t>(b[2]) << 32 | static_cast<uint64_t>(b[3]) << 48;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (i + r < s.ni) out[r] = b[r];
+  }
+}
+__global__ __launch_bounds__(256) void vocab_join_kernel(const VocabSums a, const VocabSums w, int blocks_a) {
+  if (static_cast<int>(blockIdx.x) < blocks_a) join_block(a, blockIdx.x);
+  else join_block(w, blockIdx.x - blocks_a);
 }
 
 template <auto kernel>
@@ -464,61 +595,86 @@ int with_lds(int lds, const char* what) {   // more LDS than the default limit o
   return NITI_OK;
 }
 
+long long tiles_of(long long ni, long long nj, int ti, int tj) { return ((ni + ti - 1) / ti) * ((nj + tj - 1) / tj); }
+
 template <class T>
 int run_stats(const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
   if (const int rc = with_lds<vocab_stats_kernel<T>>(T::kLds, "vocab_stats")) return rc;
-  const long long tiles = static_cast<long long>((l.classes + T::TI - 1) / T::TI) * ((l.rows + T::TJ - 1) / T::TJ);
+  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ);
+  if (tiles > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: %lld tiles", tiles);
   hipLaunchKernelGGL(vocab_stats_kernel<T>, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, l, s);
   return check_launch("vocab_stats");
 }
 template <class T>
 int run_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
   if (const int rc = with_lds<vocab_grad_kernel<T>>(T::kLds, "vocab_grad")) return rc;
-  const long long tiles = static_cast<long long>((l.classes + T::TI - 1) / T::TI) * ((l.rows + T::TJ - 1) / T::TJ);
+  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ) + g.widen.blocks;
+  if (tiles > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_grad: %lld tiles", tiles);
   hipLaunchKernelGGL(vocab_grad_kernel<T>, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, l, g);
   return check_launch("vocab_grad");
 }
-template <class T, bool kYSlow>
-int run_sums(const VocabSums& s, hipStream_t stream) {
-  if (const int rc = with_lds<vocab_sums_kernel<T, kYSlow>>(T::kLds, "vocab_sums")) return rc;
-  const long long tiles = static_cast<long long>((s.ni + T::TI - 1) / T::TI) * ((s.nj + T::TJ - 1) / T::TJ) * s.slices;
-  hipLaunchKernelGGL((vocab_sums_kernel<T, kYSlow>), dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, s);
+template <class TA, class TW>
+int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
+  constexpr int kLds = TA::kLds > TW::kLds ? TA::kLds : TW::kLds;
+  if (const int rc = with_lds<vocab_sums_kernel<TA, TW>>(kLds, "vocab_sums")) return rc;
+  const long long na = (tiles_of(a.ni, a.nj, TA::TI, TA::TJ) * a.slices + 7) / 8 * 8, nw = tiles_of(w.ni, w.nj, TW::TI, TW::TJ) * w.slices;
+  if (na + nw > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_sums: %lld tiles", na + nw);
+  hipLaunchKernelGGL((vocab_sums_kernel<TA, TW>), dim3(static_cast<unsigned>(na + nw)), dim3(TA::kThreads), kLds, stream, a, w, static_cast<int>(na));
   return check_launch("vocab_sums");
 }
 
-long long tiles_of(long long ni, long long nj, int ti, int tj) { return ((ni + ti - 1) / ti) * ((nj + tj - 1) / tj); }
-bool large_tiles(int ni, int nj) { return tiles_of(ni, nj, 256, 256) >= 200; }
-
 }  // namespace
 
-int launch_vocab_stats(const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
-  return l.rows <= 32 ? run_stats<TileFew>(l, s, stream) : run_stats<TileLarge>(l, s, stream);
+// Time of a round of large tiles (one per unit) to one of middle tiles (two per unit), for equal reductions: 1.2 to 0.7.
+VocabTile vocab_logits_tile(int rows, int classes) {
+  if (rows <= 32) return kVocabFew;
+  const double large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256) * 1.2;
+  const double middle = static_cast<double>((tiles_of(classes, rows, 128, 128) + 511) / 512) * 0.7;
+  return large <= middle ? kVocabLarge : kVocabMiddle;
 }
 
-int launch_vocab_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
-  if (l.rows <= 32) return run_grad<TileFew>(l, g, stream);
-  return large_tiles(l.classes, l.rows) ? run_grad<TileLarge>(l, g, stream) : run_grad<TileMiddle>(l, g, stream);
+int vocab_stats_tiles(VocabTile t, int classes) { return t == kVocabLarge ? (classes + 255) / 256 : (classes + 127) / 128; }
+
+int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
+  return t == kVocabFew ? run_stats<TileFew>(l, s, stream) : (t == kVocabLarge ? run_stats<TileLarge>(l, s, stream) : run_stats<TileMiddle>(l, s, stream));
 }
 
-void vocab_sums_plan(int ni, int nj, int nk, int* slices, int* steps) {
-  const long long tiles = nj <= 32 ? tiles_of(ni, nj, 256, 32) : (large_tiles(ni, nj) ? tiles_of(ni, nj, 256, 256) : tiles_of(ni, nj, 128, 128));
-  const int stages = (nk + 63) / 64;
-  long long want = tiles >= 200 ? 1 : (512 + tiles - 1) / tiles;
-  if (want > stages / 4) want = stages / 4;
-  if (want < 1) want = 1;
-  *steps = static_cast<int>((stages + want - 1) / want);
-  *slices = (stages + *steps - 1) / *steps;
+// a tile looks through the places of all of its rows: up to sixteen rounds of its threads
+bool vocab_grad_writes_targets(VocabTile t, int top) { return top <= (t == kVocabLarge ? 4 : (t == kVocabMiddle ? 32 : 128)); }
+
+int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
+  return t == kVocabFew ? run_grad<TileFew>(l, g, stream) : (t == kVocabLarge ? run_grad<TileLarge>(l, g, stream) : run_grad<TileMiddle>(l, g, stream));
 }
 
-int launch_vocab_sums(const VocabSums& s, bool y_slow, hipStream_t stream) {
-  if (s.nj <= 32) return y_slow ? run_sums<TileFew, true>(s, stream) : run_sums<TileFew, false>(s, stream);
-  if (large_tiles(s.ni, s.nj)) return y_slow ? run_sums<TileLarge, true>(s, stream) : run_sums<TileLarge, false>(s, stream);
-  return y_slow ? run_sums<TileMiddle, true>(s, stream) : run_sums<TileMiddle, false>(s, stream);
+VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w) {
+  const long long large = tiles_of(features, rows, 256, 256) + tiles_of(features, classes, 256, 256);
+  const VocabTile t = rows <= 32 ? kVocabFew : (large >= 256 ? kVocabLarge : kVocabMiddle);
+  const long long na = t == kVocabFew ? tiles_of(features, rows, 128, 32) : (t == kVocabLarge ? tiles_of(features, rows, 256, 256) : tiles_of(features, rows, 128, 128));
+  const long long nw = t == kVocabLarge ? tiles_of(features, classes, 256, 256) : tiles_of(features, classes, 128, 128);
+  const int sa = (classes + 63) / 64, sw = (rows + 63) / 64;
+  // a workgroup's share of all stages, were they spread evenly: no tile is longer, none is cut below eight stages
+  long long share = (na * sa + nw * sw) / (t == kVocabLarge ? 256 : 512) + 1;
+  if (share < 8) share = 8;
+  const auto cut = [share](int stages, int* slices, int* steps) {
+    const long long want = (stages + share - 1) / share;
+    *steps = static_cast<int>((stages + want - 1) / want);
+    *slices = (stages + *steps - 1) / *steps;
+  };
+  cut(sa, slices_a, steps_a);
+  cut(sw, slices_w, steps_w);
+  return t;
 }
 
-int launch_vocab_join(const VocabSums& s, hipStream_t stream) {
-  const long long quads = static_cast<long long>((s.ni + 3) / 4) * s.nj;
-  hipLaunchKernelGGL(vocab_join_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, stream, s);
+int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream) {
+  return t == kVocabFew ? run_sums<TileFew, TileMiddle>(a, w, stream)
+                        : (t == kVocabLarge ? run_sums<TileLarge, TileLarge>(a, w, stream) : run_sums<TileMiddle, TileMiddle>(a, w, stream));
+}
+
+int launch_vocab_join(const VocabSums* a, const VocabSums* w, hipStream_t stream) {
+  const auto blocks = [](const VocabSums* s) { return s == nullptr ? 0 : (static_cast<long long>((s->ni + 3) / 4) * s->nj + 255) / 256; };
+  const long long na = blocks(a), nw = blocks(w);
+  if (na + nw > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_join: %lld workgroups", na + nw);
+  hipLaunchKernelGGL(vocab_join_kernel, dim3(static_cast<unsigned>(na + nw)), dim3(256), 0, stream, a != nullptr ? *a : *w, w != nullptr ? *w : *a, static_cast<int>(na));
   return check_launch("vocab_join");
 }
 

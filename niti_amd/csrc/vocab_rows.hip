@@ -1,9 +1,10 @@
 // Losses over a large vocabulary (vocab.h): what is done per row, the operands' layouts, and the entry points.
 //
-//   forward:  statistics of the logits per row and kVocabClassTile classes (vocab.hip), then a wavefront per row joins them, multiplies out the logits
-//             of the row's targets, and leaves loss, logarithm of the denominator and what the backward pass wants to know
+//   forward:  statistics of the logits per row and tile of classes (vocab.hip), then a wavefront per row joins them, multiplies out the
+//             logits of the row's targets, and leaves loss, logarithm of the denominator and what the backward pass wants to know
 //   backward: a piece of the classes after the other: the piece's softmax as 16-bit floats (vocab.hip), the targets' places
-//             overwritten with their gradient (known in 32 bits: a small difference p - q keeps its digits), both products
+//             overwritten with their gradient (known in 32 bits: a small difference p - q keeps its digits), both products in one launch,
+//             their slices added in another
 #include <math.h>
 
 #include "vocab.h"
@@ -13,67 +14,43 @@ namespace {
 
 constexpr int kMaxFeatures = 65536;      // |s| <= 2^30: differences of two logits are int32
 constexpr long long kPieceMost = 1LL << 20;
-constexpr long long kPieceGrad = 64LL << 20;    // elements of the gradient's piece
-constexpr long long kPieceWide = 128LL << 20;   // elements of the weights' 16-bit piece
+constexpr long long kPieceGrad = 64LL << 20;    // elements of the gradient's piece: 128 MiB, half of the last-level cache
 
 long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
 
 // ---- layouts -------------------------------------------------------------------------------------------------------
-// rows of `n` bytes at any address and pitch -> rows of a multiple of 16, zero behind the last byte
-__global__ __launch_bounds__(256) void vocab_pad_kernel(const int8_t* __restrict__ src, long long pitch, int8_t* __restrict__ dst, long long rows, int n) {
+// Rows of `n` bytes at any address and pitch -> rows of a multiple of 16, zero behind the last byte; up to two matrices in a launch.  Reads
+// whole words that hold at least one byte of the row, and puts sixteen bytes together from five of them.
+struct VocabPad {
+  const int8_t* src;
+  long long pitch;
+  int8_t* dst;
+  long long rows;
+  int blocks;
+};
+__global__ __launch_bounds__(256) void vocab_pad_kernel(const VocabPad a, const VocabPad b, int n) {
+  const bool first = static_cast<int>(blockIdx.x) < a.blocks;
+  const VocabPad p = first ? a : b;
   const int pieces = (n + 15) / 16;
-  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= rows * pieces) return;
+  const long long at = static_cast<long long>(blockIdx.x - (first ? 0 : a.blocks)) * 256 + threadIdx.x;
+  if (at >= p.rows * pieces) return;
   const long long row = at / pieces;
   const int c = static_cast<int>(at - row * pieces) * 16;
-  union {
-    int8_t b[16];
-    v4i v;
-  } u;
+  const uintptr_t from = reinterpret_cast<uintptr_t>(p.src + row * p.pitch + c);
+  const uint32_t* const words = reinterpret_cast<const uint32_t*>(from & ~static_cast<uintptr_t>(3));
+  const int skip = static_cast<int>(from & 3), bytes = min(16, n - c);
+  uint32_t w[5];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) u.b[i] = c + i < n ? src[row * pitch + c + i] : static_cast<int8_t>(0);
-  *reinterpret_cast<v4i*>(dst + at * 16) = u.v;
-}
-
-// int8 rows (16-byte aligned, `n` values, zero up to the next multiple of 16) -> 16-bit floats, times weight / 2^*exponent 2^kRowExponent
-// of the row where there are weights
-__global__ __launch_bounds__(256) void vocab_widen_kernel(const int8_t* __restrict__ src, long long src_pitch, _Float16* __restrict__ dst, long long pitch,
-                                                          long long rows, int n, const float* __restrict__ weight, const int32_t* __restrict__ exponent) {
-  const int pieces = (n + 15) / 16;
-  const long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= rows * pieces) return;
-  const long long row = at / pieces;
-  const int c = static_cast<int>(at - row * pieces) * 16;
-  union {
-    int8_t b[16];
-    v4i v;
-  } u;
-  u.v = *reinterpret_cast<const v4i*>(src + row * src_pitch + c);
-  float scale = 1.0f;
-  if (weight != nullptr) scale = ldexpf(weight[row], kRowExponent - *exponent);
-  _Float16 o[16];
+  for (int i = 0; i < 5; ++i) w[i] = 4 * i < skip + bytes ? words[i] : 0u;
+  v4i o;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = static_cast<_Float16>(static_cast<float>(u.b[i]) * scale);
-  v4i* const out = reinterpret_cast<v4i*>(dst + row * pitch + c);
-  out[0] = *reinterpret_cast<v4i*>(&o[0]);
-  out[1] = *reinterpret_cast<v4i*>(&o[8]);
-}
-
-// smallest power of two above every weight's magnitude, as an exponent; one workgroup
-__global__ __launch_bounds__(1024) void vocab_weight_exponent_kernel(const float* __restrict__ weight, int n, int32_t* __restrict__ exponent) {
-  __shared__ float most[16];
-  float m = 0.0f;
-  for (int i = threadIdx.x; i < n; i += 1024) m = fmaxf(m, fabsf(weight[i]));
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) m = fmaxf(m, most[i]);
-    int e = 0;
-    if (m > 0.0f) frexpf(fminf(m, 3.402823466e38f), &e);
-    *exponent = e;
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v = static_cast<uint32_t>(((static_cast<uint64_t>(w[i + 1]) << 32) | w[i]) >> (8 * skip));
+    const int in = bytes - 4 * i;       // bytes of this word that are the row's
+    if (in < 4) v &= in <= 0 ? 0u : (1u << (8 * in)) - 1u;
+    o[i] = static_cast<int>(v);
   }
+  *reinterpret_cast<v4i*>(p.dst + at * 16) = o;
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
@@ -258,6 +235,7 @@ struct Layout {
 struct ForwardPlan {
   size_t a, w, part, bytes;
   bool copy_a, copy_w;
+  VocabTile tile;
   int tiles;
 };
 ForwardPlan forward_plan(const Matrix& a, const Matrix& w, int features) {
@@ -268,16 +246,18 @@ ForwardPlan forward_plan(const Matrix& a, const Matrix& w, int features) {
   p.copy_w = needs_copy(w, features);
   p.a = l.take(p.copy_a ? a.rows * row : 0);
   p.w = l.take(p.copy_w ? w.rows * row : 0);
-  p.tiles = static_cast<int>((w.rows + kVocabClassTile - 1) / kVocabClassTile);
+  p.tile = vocab_logits_tile(static_cast<int>(a.rows), static_cast<int>(w.rows));
+  p.tiles = vocab_stats_tiles(p.tile, static_cast<int>(w.rows));
   p.part = l.take(a.rows * p.tiles * 8);
   p.bytes = l.bytes;
   return p;
 }
 
 struct BackwardPlan {
-  size_t a, w, wide_a, wide_w, grad, part_a, part_w, exponent, bytes;
+  size_t a, w, wide, grad, part_a, part_w, exponent, bytes;
   bool copy_a, copy_w;
   long long piece, pitch16, part_pitch;   // classes at a time; values of a 16-bit row; values of a partial sum's row
+  VocabTile tile;
   int slices_a, steps_a, slices_w, steps_w;
   bool parts_a, parts_w;
 };
@@ -290,20 +270,17 @@ BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
   p.pitch16 = row;
   p.part_pitch = round_up(features, 4);
   long long piece = kPieceGrad / a.rows;
-  if (piece > kPieceWide / features) piece = kPieceWide / features;
   if (piece < 4096) piece = 4096;
   if (piece > kPieceMost) piece = kPieceMost;
-  piece = piece / kVocabClassTile * kVocabClassTile;
+  piece = piece / 256 * 256;
   if (piece > round_up(w.rows, 8)) piece = round_up(w.rows, 8);
   p.piece = piece;
-  vocab_sums_plan(features, static_cast<int>(a.rows), static_cast<int>(piece), &p.slices_a, &p.steps_a);
-  vocab_sums_plan(features, static_cast<int>(piece), static_cast<int>(a.rows), &p.slices_w, &p.steps_w);
+  p.tile = vocab_sums_plan(static_cast<int>(a.rows), features, static_cast<int>(piece), &p.slices_a, &p.steps_a, &p.slices_w, &p.steps_w);
   p.parts_a = p.slices_a > 1 || piece < w.rows;
   p.parts_w = p.slices_w > 1;
   p.a = l.take(p.copy_a ? a.rows * row : 0);
   p.w = l.take(p.copy_w ? w.rows * row : 0);
-  p.wide_a = l.take(a.rows * p.pitch16 * 2);
-  p.wide_w = l.take(piece * p.pitch16 * 2);
+  p.wide = l.take(a.rows * p.pitch16 * 2);
   p.grad = l.take(a.rows * piece * 2);
   p.part_a = l.take(p.parts_a ? p.slices_a * a.rows * p.part_pitch * 4 : 0);
   p.part_w = l.take(p.parts_w ? p.slices_w * piece * p.part_pitch * 4 : 0);
@@ -312,16 +289,17 @@ BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
   return p;
 }
 
-int pad_rows(const Matrix& m, int features, int8_t* dst, hipStream_t stream) {
-  const long long n = m.rows * ((features + 15) / 16);
-  hipLaunchKernelGGL(vocab_pad_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, stream, m.p, m.pitch, dst, m.rows, features);
+// copies what cannot be read in place, and points a and w at the copies
+int pad_rows(Matrix* a, bool copy_a, int8_t* to_a, Matrix* w, bool copy_w, int8_t* to_w, int features, hipStream_t stream) {
+  if (!copy_a && !copy_w) return NITI_OK;
+  const auto pad = [features](const Matrix& m, bool copy, int8_t* to) {
+    return VocabPad{m.p, m.pitch, to, m.rows, copy ? static_cast<int>((m.rows * ((features + 15) / 16) + 255) / 256) : 0};
+  };
+  const VocabPad pa = pad(*a, copy_a, to_a), pw = pad(*w, copy_w, to_w);
+  hipLaunchKernelGGL(vocab_pad_kernel, dim3(static_cast<unsigned>(pa.blocks) + static_cast<unsigned>(pw.blocks)), dim3(256), 0, stream, pa, pw, features);
+  if (copy_a) *a = Matrix{to_a, round_up(features, 16), a->rows};
+  if (copy_w) *w = Matrix{to_w, round_up(features, 16), w->rows};
   return check_launch("vocab_pad");
-}
-int widen_rows(const Matrix& m, int features, _Float16* dst, long long pitch, const float* weight, const int32_t* exponent, hipStream_t stream) {
-  const long long n = m.rows * ((features + 15) / 16);
-  hipLaunchKernelGGL(vocab_widen_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, stream, m.p, m.pitch, dst, pitch, m.rows, features, weight,
-                     exponent);
-  return check_launch("vocab_widen");
 }
 VocabOperand bytes_operand(const Matrix& m, int features) {
   return VocabOperand{m.p, m.pitch, static_cast<int>(m.rows), static_cast<int>(round_up(features, 16))};
@@ -351,17 +329,10 @@ int forward(const char* who, const int8_t* act, long long act_pitch, const int8_
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
     return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
   char* const ws = static_cast<char*>(workspace);
-  if (p.copy_a) {
-    if (const int rc = pad_rows(a, features, reinterpret_cast<int8_t*>(ws + p.a), stream)) return rc;
-    a = Matrix{reinterpret_cast<int8_t*>(ws + p.a), round_up(features, 16), rows};
-  }
-  if (p.copy_w) {
-    if (const int rc = pad_rows(b, features, reinterpret_cast<int8_t*>(ws + p.w), stream)) return rc;
-    b = Matrix{reinterpret_cast<int8_t*>(ws + p.w), round_up(features, 16), classes};
-  }
+  if (const int rc = pad_rows(&a, p.copy_a, reinterpret_cast<int8_t*>(ws + p.a), &b, p.copy_w, reinterpret_cast<int8_t*>(ws + p.w), features, stream)) return rc;
   int2* const part = reinterpret_cast<int2*>(ws + p.part);
   const VocabLogits l{bytes_operand(b, features), bytes_operand(a, features), classes, rows, features, exp_a, exp_w, 1.0f / t};
-  if (const int rc = launch_vocab_stats(l, VocabStats{part, p.tiles}, stream)) return rc;
+  if (const int rc = launch_vocab_stats(p.tile, l, VocabStats{part, p.tiles}, stream)) return rc;
   const VocabRows r{part, p.tiles, a.p, b.p, a.pitch, b.pitch, rows, classes, (features + 15) / 16, exp_a, exp_w, t, index, index_bytes, ignored, value, value_type,
                     top, loss, lse, state};
   hipLaunchKernelGGL(vocab_rows_kernel, dim3((rows + 3) / 4), dim3(256), 4 * 12 * top, stream, r);
@@ -420,51 +391,42 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
     return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
   char* const ws = static_cast<char*>(workspace);
-  if (p.copy_a) {
-    if (const int rc = pad_rows(a, features, reinterpret_cast<int8_t*>(ws + p.a), st)) return rc;
-    a = Matrix{reinterpret_cast<int8_t*>(ws + p.a), round_up(features, 16), rows};
-  }
-  if (p.copy_w) {
-    if (const int rc = pad_rows(b, features, reinterpret_cast<int8_t*>(ws + p.w), st)) return rc;
-    b = Matrix{reinterpret_cast<int8_t*>(ws + p.w), round_up(features, 16), classes};
-  }
-  _Float16* const wide_a = reinterpret_cast<_Float16*>(ws + p.wide_a);
-  _Float16* const wide_w = reinterpret_cast<_Float16*>(ws + p.wide_w);
+  if (const int rc = pad_rows(&a, p.copy_a, reinterpret_cast<int8_t*>(ws + p.a), &b, p.copy_w, reinterpret_cast<int8_t*>(ws + p.w), features, st)) return rc;
+  _Float16* const wide = reinterpret_cast<_Float16*>(ws + p.wide);
   _Float16* const grad = reinterpret_cast<_Float16*>(ws + p.grad);
   int32_t* const exponent = reinterpret_cast<int32_t*>(ws + p.exponent);
   // weights of the rows go into the activations' 16-bit copy (their sum over the rows is one product); one weight for all into the result
   const bool each = weight != nullptr && weights == rows && rows > 1;
-  if (each) {
-    hipLaunchKernelGGL(vocab_weight_exponent_kernel, dim3(1), dim3(1024), 0, st, weight, rows, exponent);
-    if (const int rc = check_launch(who)) return rc;
-  }
-  if (const int rc = widen_rows(a, features, wide_a, p.pitch16, each ? weight : nullptr, exponent, st)) return rc;
+  const long long quarter_rows = (rows * round_up(features, 16) / 16 + 511) / 512;
 
   for (long long first = 0; first < classes; first += p.piece) {
     const int here = static_cast<int>(classes - first < p.piece ? classes - first : p.piece);
     const Matrix piece{b.p + first * b.pitch, b.pitch, here};
-    if (const int rc = widen_rows(piece, features, wide_w, p.pitch16, nullptr, nullptr, st)) return rc;
     const VocabLogits l{bytes_operand(piece, features), bytes_operand(a, features), here, rows, features, exp_a, exp_w, 1.0f / temperature};
-    if (const int rc = launch_vocab_grad(l, VocabGrad{state, vocab_state_words(top), grad, p.piece}, st)) return rc;
-    const long long places = static_cast<long long>(rows) * top;
-    hipLaunchKernelGGL(vocab_targets_kernel, dim3(static_cast<unsigned>((places + 255) / 256)), dim3(256), 0, st, state, rows, top, first, here, grad, p.piece);
-    if (const int rc = check_launch(who)) return rc;
+    const VocabTile tile = vocab_logits_tile(rows, here);
+    const bool targets = vocab_grad_writes_targets(tile, top);
+    const VocabWiden widen{a.p, a.pitch, wide, p.pitch16, rows, features, each ? weight : nullptr, exponent,
+                           first == 0 ? static_cast<int>(quarter_rows < 512 ? quarter_rows : 512) : 0};
+    if (const int rc = launch_vocab_grad(tile, l, VocabGrad{state, vocab_state_words(top), targets ? top : 0, first, grad, p.piece, widen}, st)) return rc;
+    if (!targets) {
+      const long long places = static_cast<long long>(rows) * top;
+      hipLaunchKernelGGL(vocab_targets_kernel, dim3(static_cast<unsigned>((places + 255) / 256)), dim3(256), 0, st, state, rows, top, first, here, grad, p.piece);
+      if (const int rc = check_launch(who)) return rc;
+    }
 
     const int stages = (here + 63) / 64;
-    VocabSums sa{VocabOperand{wide_w, p.pitch16 * 2, here, 0}, VocabOperand{grad, p.piece * 2, rows, static_cast<int>(round_up(here, 8) * 2)}, features, rows, here,
-                 (stages + p.steps_a - 1) / p.steps_a, p.steps_a, p.parts_a ? reinterpret_cast<float*>(ws + p.part_a) : nullptr, p.part_pitch, first > 0 ? 1 : 0, d_act,
-                 temperature, exp_w, -kGradExponent, nullptr, weight, weights};
-    if (const int rc = launch_vocab_sums(sa, false, st)) return rc;
-    VocabSums sw{VocabOperand{wide_a, p.pitch16 * 2, rows, 0}, VocabOperand{grad, p.piece * 2, rows, 0}, features, here, rows, p.slices_w, p.steps_w,
-                 p.parts_w ? reinterpret_cast<float*>(ws + p.part_w) : nullptr, p.part_pitch, 0, d_w + first * features, temperature, exp_a,
-                 -kGradExponent - (each ? kRowExponent : 0), each ? exponent : nullptr, each ? nullptr : weight, 1};
-    if (const int rc = launch_vocab_sums(sw, true, st)) return rc;
-    if (p.parts_w) {
-      if (const int rc = launch_vocab_join(sw, st)) return rc;
-    }
-    if (p.parts_a && first + p.piece >= classes) {
-      sa.slices = p.slices_a;
-      if (const int rc = launch_vocab_join(sa, st)) return rc;
+    VocabSums sa{VocabOperand{piece.p, piece.pitch, here, static_cast<int>(round_up(features, 16))},
+                 VocabOperand{grad, p.piece * 2, rows, static_cast<int>(round_up(here, 8) * 2)}, features, rows, here, (stages + p.steps_a - 1) / p.steps_a, p.steps_a,
+                 p.parts_a ? reinterpret_cast<float*>(ws + p.part_a) : nullptr, p.part_pitch, first > 0 ? 1 : 0, d_act, temperature, exp_w, -kGradExponent, nullptr,
+                 weight, weights};
+    const VocabSums sw{VocabOperand{wide, p.pitch16 * 2, rows, static_cast<int>(p.pitch16 * 2)}, VocabOperand{grad, p.piece * 2, rows, static_cast<int>(p.piece * 2)},
+                       features, here, rows, p.slices_w, p.steps_w, p.parts_w ? reinterpret_cast<float*>(ws + p.part_w) : nullptr, p.part_pitch, 0,
+                       d_w + first * features, temperature, exp_a, -kGradExponent - (each ? kRowExponent : 0), each ? exponent : nullptr, each ? nullptr : weight, 1};
+    if (const int rc = launch_vocab_sums(p.tile, sa, sw, st)) return rc;
+    const bool join_a = p.parts_a && first + p.piece >= classes;
+    sa.slices = p.slices_a;
+    if (join_a || p.parts_w) {
+      if (const int rc = launch_vocab_join(join_a ? &sa : nullptr, p.parts_w ? &sw : nullptr, st)) return rc;
     }
   }
   return NITI_OK;
