@@ -70,7 +70,7 @@ struct VocabGrad {           // sum_j q_j p, times 2^kGradExponent, of the class
   long long first;           // class that the piece starts at
   _Float16* g;               // [rows][pitch], zero between the piece's last class and the next multiple of eight
   long long pitch;
-  VocabWiden widen;          // done by workgroups of its own
+  VocabWiden widen_a, widen_w;   // done by workgroups of their own
 };
 
 struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
@@ -93,10 +93,11 @@ struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
 enum VocabTile { kVocabLarge, kVocabMiddle, kVocabFew };
 VocabTile vocab_logits_tile(int rows, int classes);
 int vocab_stats_tiles(VocabTile t, int classes);    // pairs that launch_vocab_stats leaves of a row
+bool vocab_sums_wants_wide_weights(VocabTile t);
 bool vocab_grad_writes_targets(VocabTile t, int top);
 int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream);
 int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hipStream_t stream);
-// Both gradients' sums of a piece: a = the activations' (x: int8 weights, reduction slow; y: the piece's gradient, reduction fast), w = the
+// Both gradients' sums of a piece: a = the activations' (x: weights, int8 or a 16-bit copy, reduction slow; y: the piece's gradient, reduction fast), w = the
 // weights' (x: 16-bit activations, y: the piece's gradient, reduction slow in both)
 VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w);
 int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream);

@@ -415,7 +415,9 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
   if (static_cast<int>(blockIdx.x) >= ti * tj) {
-    widen_block(g.widen, blockIdx.x - ti * tj, T::kThreads, smem);
+    const int block = blockIdx.x - ti * tj;
+    if (block < g.widen_a.blocks) widen_block(g.widen_a, block, T::kThreads, smem);
+    else widen_block(g.widen_w, block - g.widen_a.blocks, T::kThreads, smem);
     return;
   }
   int bi, bj;
@@ -538,12 +540,14 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
   }
 }
 
-// Both gradients' sums: the first `blocks_a` workgroups (a multiple of eight, see tile_of) the activations', the others the weights'.
+// Both gradients' sums: the first `blocks_a` workgroups (a multiple of eight, see tile_of) the activations', the others the weights'.  The
+// large tile reads a 16-bit copy of the int8 weights: made 16-bit in registers its fragments take 487 us of 8192 x 8192 x 4096, read from
+// the copy 435, and the copy is 20 us of workgroups in the shadow of another launch.
 template <class TA, class TW>
 __global__ __launch_bounds__(TA::kThreads, TA::kPerUnit) void vocab_sums_kernel(const VocabSums a, const VocabSums w, int blocks_a) {
   static_assert(TA::kThreads == TW::kThreads, "one launch");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  if (static_cast<int>(blockIdx.x) < blocks_a) sums_tile<TA, kSlow8, kFast>(a, blockIdx.x, smem);
+  if (static_cast<int>(blockIdx.x) < blocks_a) sums_tile<TA, TA::TI == 256 ? kSlow16 : kSlow8, kFast>(a, blockIdx.x, smem);
   else sums_tile<TW, kSlow16, kSlow16>(w, blockIdx.x - blocks_a, smem);
 }
 
@@ -608,7 +612,7 @@ int run_stats(const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
 template <class T>
 int run_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
   if (const int rc = with_lds<vocab_grad_kernel<T>>(T::kLds, "vocab_grad")) return rc;
-  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ) + g.widen.blocks;
+  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ) + g.widen_a.blocks + g.widen_w.blocks;
   if (tiles > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_grad: %lld tiles", tiles);
   hipLaunchKernelGGL(vocab_grad_kernel<T>, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, l, g);
   return check_launch("vocab_grad");
@@ -638,6 +642,8 @@ int vocab_stats_tiles(VocabTile t, int classes) { return t == kVocabLarge ? (cla
 int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
   return t == kVocabFew ? run_stats<TileFew>(l, s, stream) : (t == kVocabLarge ? run_stats<TileLarge>(l, s, stream) : run_stats<TileMiddle>(l, s, stream));
 }
+
+bool vocab_sums_wants_wide_weights(VocabTile t) { return t == kVocabLarge; }
 
 // a tile looks through the places of all of its rows: up to sixteen rounds of its threads
 bool vocab_grad_writes_targets(VocabTile t, int top) { return top <= (t == kVocabLarge ? 4 : (t == kVocabMiddle ? 32 : 128)); }

@@ -15,6 +15,7 @@ namespace {
 constexpr int kMaxFeatures = 65536;      // |s| <= 2^30: differences of two logits are int32
 constexpr long long kPieceMost = 1LL << 20;
 constexpr long long kPieceGrad = 64LL << 20;    // elements of the gradient's piece: 128 MiB, half of the last-level cache
+constexpr long long kPieceWide = 128LL << 20;   // elements of the weights' 16-bit copy
 
 long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
 
@@ -254,7 +255,7 @@ ForwardPlan forward_plan(const Matrix& a, const Matrix& w, int features) {
 }
 
 struct BackwardPlan {
-  size_t a, w, wide, grad, part_a, part_w, exponent, bytes;
+  size_t a, w, wide_a, wide_w, grad, part_a, part_w, exponent, bytes;
   bool copy_a, copy_w;
   long long piece, pitch16, part_pitch;   // classes at a time; values of a 16-bit row; values of a partial sum's row
   VocabTile tile;
@@ -270,6 +271,7 @@ BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
   p.pitch16 = row;
   p.part_pitch = round_up(features, 4);
   long long piece = kPieceGrad / a.rows;
+  if (a.rows > 32 && piece > kPieceWide / features) piece = kPieceWide / features;
   if (piece < 4096) piece = 4096;
   if (piece > kPieceMost) piece = kPieceMost;
   piece = piece / 256 * 256;
@@ -280,7 +282,8 @@ BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
   p.parts_w = p.slices_w > 1;
   p.a = l.take(p.copy_a ? a.rows * row : 0);
   p.w = l.take(p.copy_w ? w.rows * row : 0);
-  p.wide = l.take(a.rows * p.pitch16 * 2);
+  p.wide_a = l.take(a.rows * p.pitch16 * 2);
+  p.wide_w = l.take(vocab_sums_wants_wide_weights(p.tile) ? piece * p.pitch16 * 2 : 0);
   p.grad = l.take(a.rows * piece * 2);
   p.part_a = l.take(p.parts_a ? p.slices_a * a.rows * p.part_pitch * 4 : 0);
   p.part_w = l.take(p.parts_w ? p.slices_w * piece * p.part_pitch * 4 : 0);
@@ -392,12 +395,17 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
     return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
   char* const ws = static_cast<char*>(workspace);
   if (const int rc = pad_rows(&a, p.copy_a, reinterpret_cast<int8_t*>(ws + p.a), &b, p.copy_w, reinterpret_cast<int8_t*>(ws + p.w), features, st)) return rc;
-  _Float16* const wide = reinterpret_cast<_Float16*>(ws + p.wide);
+  _Float16* const wide_a = reinterpret_cast<_Float16*>(ws + p.wide_a);
+  _Float16* const wide_w = reinterpret_cast<_Float16*>(ws + p.wide_w);
+  const bool wide_weights = vocab_sums_wants_wide_weights(p.tile);
   _Float16* const grad = reinterpret_cast<_Float16*>(ws + p.grad);
   int32_t* const exponent = reinterpret_cast<int32_t*>(ws + p.exponent);
   // weights of the rows go into the activations' 16-bit copy (their sum over the rows is one product); one weight for all into the result
   const bool each = weight != nullptr && weights == rows && rows > 1;
-  const long long quarter_rows = (rows * round_up(features, 16) / 16 + 511) / 512;
+  const auto widen_blocks = [features](long long n) {      // 512 lanes of sixteen values, at most two workgroups per unit
+    const long long blocks = (n * round_up(features, 16) / 16 + 511) / 512;
+    return static_cast<int>(blocks < 512 ? blocks : 512);
+  };
 
   for (long long first = 0; first < classes; first += p.piece) {
     const int here = static_cast<int>(classes - first < p.piece ? classes - first : p.piece);
@@ -405,9 +413,9 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
     const VocabLogits l{bytes_operand(piece, features), bytes_operand(a, features), here, rows, features, exp_a, exp_w, 1.0f / temperature};
     const VocabTile tile = vocab_logits_tile(rows, here);
     const bool targets = vocab_grad_writes_targets(tile, top);
-    const VocabWiden widen{a.p, a.pitch, wide, p.pitch16, rows, features, each ? weight : nullptr, exponent,
-                           first == 0 ? static_cast<int>(quarter_rows < 512 ? quarter_rows : 512) : 0};
-    if (const int rc = launch_vocab_grad(tile, l, VocabGrad{state, vocab_state_words(top), targets ? top : 0, first, grad, p.piece, widen}, st)) return rc;
+    const VocabWiden widen_a{a.p, a.pitch, wide_a, p.pitch16, rows, features, each ? weight : nullptr, exponent, first == 0 ? widen_blocks(rows) : 0};
+    const VocabWiden widen_w{piece.p, piece.pitch, wide_w, p.pitch16, here, features, nullptr, nullptr, wide_weights ? widen_blocks(here) : 0};
+    if (const int rc = launch_vocab_grad(tile, l, VocabGrad{state, vocab_state_words(top), targets ? top : 0, first, grad, p.piece, widen_a, widen_w}, st)) return rc;
     if (!targets) {
       const long long places = static_cast<long long>(rows) * top;
       hipLaunchKernelGGL(vocab_targets_kernel, dim3(static_cast<unsigned>((places + 255) / 256)), dim3(256), 0, st, state, rows, top, first, here, grad, p.piece);
@@ -415,11 +423,12 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
     }
 
     const int stages = (here + 63) / 64;
-    VocabSums sa{VocabOperand{piece.p, piece.pitch, here, static_cast<int>(round_up(features, 16))},
+    VocabSums sa{wide_weights ? VocabOperand{wide_w, p.pitch16 * 2, here, static_cast<int>(p.pitch16 * 2)}
+                              : VocabOperand{piece.p, piece.pitch, here, static_cast<int>(p.pitch16)},
                  VocabOperand{grad, p.piece * 2, rows, static_cast<int>(round_up(here, 8) * 2)}, features, rows, here, (stages + p.steps_a - 1) / p.steps_a, p.steps_a,
                  p.parts_a ? reinterpret_cast<float*>(ws + p.part_a) : nullptr, p.part_pitch, first > 0 ? 1 : 0, d_act, temperature, exp_w, -kGradExponent, nullptr,
                  weight, weights};
-    const VocabSums sw{VocabOperand{wide, p.pitch16 * 2, rows, static_cast<int>(p.pitch16 * 2)}, VocabOperand{grad, p.piece * 2, rows, static_cast<int>(p.piece * 2)},
+    const VocabSums sw{VocabOperand{wide_a, p.pitch16 * 2, rows, static_cast<int>(p.pitch16 * 2)}, VocabOperand{grad, p.piece * 2, rows, static_cast<int>(p.piece * 2)},
                        features, here, rows, p.slices_w, p.steps_w, p.parts_w ? reinterpret_cast<float*>(ws + p.part_w) : nullptr, p.part_pitch, 0,
                        d_w + first * features, temperature, exp_a, -kGradExponent - (each ? kRowExponent : 0), each ? exponent : nullptr, each ? nullptr : weight, 1};
     if (const int rc = launch_vocab_sums(p.tile, sa, sw, st)) return rc;
