@@ -26,18 +26,19 @@ constexpr int kNone = -2147483647 - 1;                // below every logit
 enum Layout { kFast, kSlow16, kSlow8 };
 constexpr int stage_bytes(int r, Layout l) { return l == kSlow8 ? 64 * r : kStageBytes * r; }
 
-template <int TI_, int TJ_, int WI_, int WJ_>
+template <int TI_, int TJ_, int WI_, int WJ_, int RING_>
 struct Tile {
-  static constexpr int TI = TI_, TJ = TJ_, WI = WI_, WJ = WJ_;
+  static constexpr int TI = TI_, TJ = TJ_, WI = WI_, WJ = WJ_, RING = RING_;     // RING: buffers
   static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
   static constexpr int BI = TI / WI / 16, BJ = TJ / WJ / 16;   // 16 x 16 blocks of a wavefront
-  static constexpr int kLds = 2 * (TI + TJ) * kStageBytes;
+  static constexpr int kLds = RING * (TI + TJ) * kStageBytes;
   // workgroups per unit that the registers are cut for: two wavefronts per SIMD at least, so that all sums are ordinary registers
-  static constexpr int kPerUnit = kWaves >= 8 ? 1 : 8 / kWaves;
+  static constexpr int kPerUnit = kWaves >= 8 ? 1 : 8 / kWaves;      // (TileDeep: one by its LDS)
 };
-typedef Tile<256, 256, 2, 4> TileLarge;
-typedef Tile<128, 128, 2, 2> TileMiddle;
-typedef Tile<128, 32, 4, 1> TileFew;
+typedef Tile<256, 256, 2, 4, 2> TileLarge;
+typedef Tile<128, 128, 2, 2, 2> TileMiddle;
+typedef Tile<128, 128, 2, 2, 4> TileDeep;      // grids that leave units with one workgroup at most: what counts is how soon the loads are out
+typedef Tile<128, 32, 4, 1, 4> TileFew;
 
 // 16-lane groups: lane i of a group names 8 bytes of a 4 x 16 block of 16-bit values (row i / 4, columns 4 (i % 4) .. + 4) and receives
 // column i of it
@@ -74,11 +75,11 @@ struct Source {
   static constexpr bool kSlow = L != kFast;
   static constexpr int kStage = stage_bytes(R, L);
   static constexpr int kInstructions = kStage / 1024;                       // of a stage
-  static constexpr int kLoads = (kInstructions + kWaves - 1) / kWaves;      // of a wavefront, 16 bytes per lane each
+  static constexpr int kLoads = kInstructions / kWaves;                     // of a wavefront, 16 bytes per lane each
   static constexpr int kRowBytes = L == kFast ? kStageBytes : (L == kSlow16 ? 2 * R : R);
   static constexpr int kRowsPerLoad = 1024 / kRowBytes;
   static constexpr int kPieces = kRowBytes / 16;
-  static_assert(kInstructions % kWaves == 0 || kInstructions < kWaves, "whole wavefronts");
+  static_assert(kInstructions % kWaves == 0, "the same number of each wavefront");
 
   const char* base;
   long long left;        // bytes from base to the end of the matrix
@@ -127,8 +128,7 @@ struct Source {
   }
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned lds, int q) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (kInstructions >= kWaves || wave < kInstructions)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, NITI_LDS_AT(lds + (q * kWaves + wave) * 1024), 16, kSlow || piece < fast_left ? voff[q] : kFar, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, NITI_LDS_AT(lds + (q * kWaves + wave) * 1024), 16, kSlow || piece < fast_left ? voff[q] : kFar, 0, 0, 0);
   }
   __device__ void next() {
     base += advance;
@@ -210,7 +210,7 @@ struct Product {
   unsigned ldsx, ldsy;
   static constexpr int kStageX = stage_bytes(T::TI, LX), kStageY = stage_bytes(T::TJ, LY);
   static constexpr int kLoadsX = Source<T::TI, LX, T::kWaves>::kLoads, kLoadsY = Source<T::TJ, LY, T::kWaves>::kLoads;
-  static_assert(2 * (kStageX + kStageY) <= T::kLds, "stages fit");
+  static_assert(T::RING * (kStageX + kStageY) <= T::kLds, "stages fit");
 
   // instruction q of a stage's loads into buffer buf
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rx, __amdgpu_buffer_rsrc_t ry, int buf, int q) const {
@@ -223,7 +223,7 @@ struct Product {
     sx.next();
     sy.next();
   }
-  // Products of half SUB; half NEXT is read in between, and where kLoad the next stage but one goes out into buffer buf, spread over the
+  // Products of half SUB; half NEXT is read in between, and where kLoad the next stage that has no buffer yet goes out into buffer buf, spread over the
   // products: a unit's loads pass at 64 bytes a clock, and a wavefront waits at a load that finds the queue full
   template <int SUB, int NEXT, bool kLoad>
   __device__ void half(int buf) {
@@ -259,7 +259,7 @@ struct Product {
   __device__ void run(const VocabOperand& x, const VocabOperand& y, int i0, int j0, int k0, int n, int x_end, int y_end, char* smem) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     ldsx = lds_addr(smem);
-    ldsy = ldsx + 2 * kStageX;
+    ldsy = ldsx + T::RING * kStageX;
     sx.init(x, i0, k0, x_end);
     sy.init(y, j0, k0, y_end);
     fx.init(ldsx, (wave / T::WJ) * T::BI);
@@ -268,11 +268,10 @@ struct Product {
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
       for (int j = 0; j < T::BJ; ++j) acc[i][j] = Acc{0, 0, 0, 0};
-    // loads of the two stages behind the last are issued like the others: they are out of range, and what they clear is not multiplied
-    issue(0);
-    issue(1);
-    constexpr int kLeast = Source<T::TI, LX, T::kWaves>::kInstructions / T::kWaves + Source<T::TJ, LY, T::kWaves>::kInstructions / T::kWaves;   // per stage
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeast) : "memory");
+    // loads of the stages behind the last are issued like the others: they are out of range, and what they clear is not multiplied
+    static_for<T::RING>([&](auto b) { issue(decltype(b)::value); });
+    constexpr int kStageLoads = kLoadsX + kLoadsY;       // of a wavefront
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::RING - 1) * kStageLoads) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     static_for<T::BJ>([&](auto j) { fy.template read<0, decltype(j)::value>(); });
@@ -283,12 +282,15 @@ struct Product {
     int buf = 0;
     for (int s = 0; s < n; ++s) {
       half<0, 1, false>(buf);
-      tile_sync();          // the next stage has landed, and this one's buffer has been read by every wavefront
-      const int step = buf == 0 ? 1 : -1;
+      // the next stage has landed, and this one's buffer has been read by every wavefront
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((T::RING - 2) * kStageLoads) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const int step = buf + 1 < T::RING ? 1 : 1 - T::RING;
       fx.other_buffer(step * kStageX);
       fy.other_buffer(step * kStageY);
       half<1, 0, true>(buf);
-      buf ^= 1;
+      buf += step;
     }
     tile_sync();            // the buffers are free
   }
@@ -632,24 +634,36 @@ int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
 // Time of a round of large tiles (one per unit) to one of middle tiles (two per unit), for equal reductions: 1.2 to 0.7.
 VocabTile vocab_logits_tile(int rows, int classes) {
   if (rows <= 32) return kVocabFew;
-  const double large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256) * 1.2;
-  const double middle = static_cast<double>((tiles_of(classes, rows, 128, 128) + 511) / 512) * 0.7;
-  return large <= middle ? kVocabLarge : kVocabMiddle;
+  const long long middle = tiles_of(classes, rows, 128, 128);
+  if (middle <= 256) return kVocabDeep;
+  const double t_large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256) * 1.2;
+  const double t_middle = static_cast<double>((middle + 511) / 512) * 0.7;
+  return t_large <= t_middle ? kVocabLarge : kVocabMiddle;
 }
 
 int vocab_stats_tiles(VocabTile t, int classes) { return t == kVocabLarge ? (classes + 255) / 256 : (classes + 127) / 128; }
 
 int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
-  return t == kVocabFew ? run_stats<TileFew>(l, s, stream) : (t == kVocabLarge ? run_stats<TileLarge>(l, s, stream) : run_stats<TileMiddle>(l, s, stream));
+  switch (t) {
+    case kVocabLarge: return run_stats<TileLarge>(l, s, stream);
+    case kVocabMiddle: return run_stats<TileMiddle>(l, s, stream);
+    case kVocabDeep: return run_stats<TileDeep>(l, s, stream);
+    default: return run_stats<TileFew>(l, s, stream);
+  }
 }
 
 bool vocab_sums_wants_wide_weights(VocabTile t) { return t == kVocabLarge; }
 
 // a tile looks through the places of all of its rows: up to sixteen rounds of its threads
-bool vocab_grad_writes_targets(VocabTile t, int top) { return top <= (t == kVocabLarge ? 4 : (t == kVocabMiddle ? 32 : 128)); }
+bool vocab_grad_writes_targets(VocabTile t, int top) { return top <= (t == kVocabLarge ? 4 : (t == kVocabFew ? 128 : 32)); }
 
 int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
-  return t == kVocabFew ? run_grad<TileFew>(l, g, stream) : (t == kVocabLarge ? run_grad<TileLarge>(l, g, stream) : run_grad<TileMiddle>(l, g, stream));
+  switch (t) {
+    case kVocabLarge: return run_grad<TileLarge>(l, g, stream);
+    case kVocabMiddle: return run_grad<TileMiddle>(l, g, stream);
+    case kVocabDeep: return run_grad<TileDeep>(l, g, stream);
+    default: return run_grad<TileFew>(l, g, stream);
+  }
 }
 
 VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w) {
@@ -658,9 +672,10 @@ VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, in
   const long long na = t == kVocabFew ? tiles_of(features, rows, 128, 32) : (t == kVocabLarge ? tiles_of(features, rows, 256, 256) : tiles_of(features, rows, 128, 128));
   const long long nw = t == kVocabLarge ? tiles_of(features, classes, 256, 256) : tiles_of(features, classes, 128, 128);
   const int sa = (classes + 63) / 64, sw = (rows + 63) / 64;
-  // a workgroup's share of all stages, were they spread evenly: no tile is longer, none is cut below eight stages
+  // a workgroup's share of all stages, were they spread evenly: no tile is longer, none is cut below sixteen stages (adding the parts is
+  // a launch of its own)
   long long share = (na * sa + nw * sw) / (t == kVocabLarge ? 256 : 512) + 1;
-  if (share < 8) share = 8;
+  if (share < 16) share = 16;
   const auto cut = [share](int stages, int* slices, int* steps) {
     const long long want = (stages + share - 1) / share;
     *steps = static_cast<int>((stages + want - 1) / want);

@@ -82,36 +82,51 @@ __device__ inline float teacher_value(const VocabRows& a, long long i) {
   return static_cast<float>(static_cast<const _Float16*>(a.value)[i]);
 }
 
-__device__ inline double wave_sum(double v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+// Sums and maxima over the wavefront by data-parallel moves (a scan inside each row of sixteen lanes, the row totals carried on), in every
+// lane: six moves of a few clocks where a shuffle through LDS is some hundred.
+template <int CTRL, int MASK>
+__device__ inline int dpp_take(int neutral, int v) { return __builtin_amdgcn_update_dpp(neutral, v, CTRL, MASK, 0xf, false); }
+template <class F>
+__device__ inline int wave_fold(int neutral, int v, F f) {
+  v = f(v, dpp_take<0x111, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x112, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x114, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x118, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x142, 0xa>(neutral, v));
+  v = f(v, dpp_take<0x143, 0xc>(neutral, v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ inline int wave_add(int v) {
+  return wave_fold(0, v, [](int a, int b) { return a + b; });
+}
+__device__ inline int wave_most(int v) {
+  return wave_fold(-2147483647 - 1, v, [](int a, int b) { return max(a, b); });
+}
+__device__ inline float wave_add(float v) {
+  return __int_as_float(wave_fold(0, __float_as_int(v), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
+}
+__device__ inline float wave_most(float v) {
+  return __int_as_float(wave_fold(__float_as_int(-INFINITY), __float_as_int(v), [](int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }));
 }
 
-// A wavefront per row.  All lanes go through every loop the same number of times: the barriers are the workgroup's.
-__global__ __launch_bounds__(256) void vocab_rows_kernel(const VocabRows a) {
+// A wavefront and workgroup per row.  The loads that depend on nothing - pairs of the tiles, exponents, targets, the row's first sixteen
+// values per lane - go out together, then those of the targets' weights, eight targets at a time: what the kernel takes is the way of these.
+__global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const bool real = blockIdx.x * 4 + wave < static_cast<unsigned>(a.rows);
-  const long long row = real ? blockIdx.x * 4 + wave : a.rows - 1;
-  float* const q = reinterpret_cast<float*>(smem) + wave * 3 * a.top;
+  const int lane = threadIdx.x;
+  const long long row = blockIdx.x;
+  float* const q = reinterpret_cast<float*>(smem);
   int* const cls = reinterpret_cast<int*>(q + a.top);
   int* const dot = cls + a.top;
-  const double k = fmin(ldexp(1.4426950408889634074 / static_cast<double>(a.t), *a.exp_a + *a.exp_w), 3.402823466e38);
-  const float kf = static_cast<float>(k);
 
+  constexpr int kHeld = 4;            // pairs in registers; a row of more tiles is read twice
   const int2* const part = a.part + row * a.tiles;
-  int m = -2147483647 - 1;
-  for (int i = lane; i < a.tiles; i += 64) m = max(m, part[i].x);
+  int2 held[kHeld];
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) m = max(m, __shfl_xor(m, off, 64));
-  double sum = 0.0;
-  for (int i = lane; i < a.tiles; i += 64) {
-    const int2 v = part[i];
-    sum += static_cast<double>(__int_as_float(v.y) * exp2f(static_cast<float>(v.x - m) * kf));
-  }
-  const double l2 = log2(wave_sum(sum));
+  for (int u = 0; u < kHeld; ++u) held[u] = lane + 64 * u < a.tiles ? part[lane + 64 * u] : make_int2(-2147483647 - 1, 0);
+  const v4i* const arow = reinterpret_cast<const v4i*>(a.a + row * a.a_pitch);
+  const v4i x0 = lane < a.pieces ? arow[lane] : v4i{0, 0, 0, 0};
+  const int exponent = *a.exp_a + *a.exp_w;
 
   // the targets and their weights
   bool bad = false;
@@ -119,86 +134,110 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(const VocabRows a) {
   for (int j = lane; j < a.top; j += 64) {
     const long long at = row * a.top + j;
     const long long c = a.index_bytes == 8 ? static_cast<const int64_t*>(a.index)[at] : static_cast<const int32_t*>(a.index)[at];
+    const float given = a.value == nullptr ? 0.0f : teacher_value(a, at) / a.t;
     const bool none = a.value == nullptr ? c == a.ignored : c < 0;
     if (!none && (c < 0 || c >= a.classes)) bad = true;
     const bool used = !none && c >= 0 && c < a.classes;
     cls[j] = used ? static_cast<int>(c) : -1;
-    const float v = !used ? -INFINITY : (a.value == nullptr ? 0.0f : teacher_value(a, at) / a.t);
+    const float v = used ? given : -INFINITY;
     q[j] = v;
     vmax = fmaxf(vmax, v);
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) vmax = fmaxf(vmax, __shfl_xor(vmax, off, 64));
-  bad = __any(bad);
-  double norm = 0.0;
-  for (int j = lane; j < a.top; j += 64) {
-    const float v = q[j];
-    const float e = v == -INFINITY ? 0.0f : expf(v - vmax);
-    q[j] = e;
-    norm += static_cast<double>(e);
-  }
-  norm = wave_sum(norm);
-  const float coef = bad ? __builtin_nanf("") : (norm > 0.0 ? 1.0f : (norm == 0.0 ? 0.0f : __builtin_nanf("")));
   __syncthreads();
 
-  // the targets' logits, four at a time
-  const v4i* const arow = reinterpret_cast<const v4i*>(a.a + row * a.a_pitch);
-  for (int j0 = 0; j0 < a.top; j0 += 4) {
-    int s[4] = {0, 0, 0, 0};
-    const v4i* w[4];
+  // the targets' logits
+  for (int j0 = 0; j0 < a.top; j0 += 8) {
+    int s[8];
+    const v4i* w[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int c = j0 + u < a.top ? cls[j0 + u] : -1;
-      w[u] = reinterpret_cast<const v4i*>(a.w + (c < 0 ? 0 : c) * a.w_pitch);   // an unused place's product is not looked at
+    for (int u = 0; u < 8; ++u) {
+      const int c = j0 + u < a.top ? __builtin_amdgcn_readfirstlane(cls[j0 + u]) : -1;
+      w[u] = c < 0 ? nullptr : reinterpret_cast<const v4i*>(a.w + c * a.w_pitch);
+      s[u] = 0;
     }
     for (int p = lane; p < a.pieces; p += 64) {
-      const v4i x = arow[p];
-      v4i y[4];
+      const v4i x = p < 64 ? x0 : arow[p];
+      v4i y[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) y[u] = w[u][p];
+      for (int u = 0; u < 8; ++u) y[u] = w[u] != nullptr ? w[u][p] : v4i{0, 0, 0, 0};
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 8; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[u] = __builtin_amdgcn_sdot4(x[i], y[u][i], s[u], false);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) s[u] += __shfl_xor(s[u], off, 64);
-      if (lane == 0 && j0 + u < a.top) dot[j0 + u] = s[u];
+    for (int u = 0; u < 8; ++u) {
+      if (j0 + u < a.top) {
+        const int all = wave_add(s[u]);
+        if (lane == 0) dot[j0 + u] = all;
+      }
     }
   }
+
+  // the denominator
+  const double k = fmin(ldexp(1.4426950408889634074 / static_cast<double>(a.t), exponent), 3.402823466e38);
+  const float kf = static_cast<float>(k);
+  int m = -2147483647 - 1;
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u) m = max(m, held[u].x);
+  for (int i = lane + 64 * kHeld; i < a.tiles; i += 64) m = max(m, part[i].x);
+  m = wave_most(m);
+  float sum = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    if (held[u].x != -2147483647 - 1) sum += __int_as_float(held[u].y) * exp2f(static_cast<float>(held[u].x - m) * kf);
+  for (int i = lane + 64 * kHeld; i < a.tiles; i += 64) {
+    const int2 v = part[i];
+    sum += __int_as_float(v.y) * exp2f(static_cast<float>(v.x - m) * kf);
+  }
+  sum = wave_add(sum);
+  int e2;
+  float mantissa = frexpf(sum, &e2);
+  if (mantissa < 0.70710678f) {
+    mantissa *= 2.0f;
+    e2 -= 1;
+  }
+  const double l2 = static_cast<double>(log2f(mantissa)) + e2;      // the float part is at most 1/2: a row that is sure of itself keeps its digits
+
+  vmax = wave_most(vmax);
+  bad = __any(bad);
+  float norm = 0.0f;
+  for (int j = lane; j < a.top; j += 64) {
+    const float v = q[j];
+    const float e = v == -INFINITY ? 0.0f : expf(v - vmax);
+    q[j] = e;
+    norm += e;
+  }
+  norm = wave_add(norm);
+  const float coef = bad ? __builtin_nanf("") : (norm > 0.0f ? 1.0f : (norm == 0.0f ? 0.0f : __builtin_nanf("")));
   __syncthreads();
 
   constexpr double kLn2 = 0.69314718055994530942;
   int32_t* const state = a.state + row * vocab_state_words(a.top);
-  double loss = 0.0;
+  float loss = 0.0f;
   for (int j = lane; j < a.top; j += 64) {
     const int c = cls[j];
     float g = 0.0f;
     bool first = c >= 0;
     if (c >= 0) {
-      const double mine = static_cast<double>(q[j]) / norm;
-      if (mine > 0.0) loss += mine * (log(mine) + kLn2 * (l2 + (static_cast<double>(m) - dot[j]) * k));
-      else if (!(mine == 0.0)) loss = mine;
+      const float mine = q[j] / norm;
+      const double behind = (static_cast<double>(dot[j]) - m) * k - l2;       // log2 of the softmax here
+      if (mine > 0.0f) loss += mine * (logf(mine) - static_cast<float>(kLn2 * behind));
+      else if (!(mine == 0.0f)) loss = mine;
       float all = 0.0f;                  // the weights of every place that names this class
       for (int i = 0; i < a.top; ++i)
         if (cls[i] == c) {
           all += q[i];
           if (i < j) first = false;      // one place speaks for all
         }
-      const float p = exp2f(static_cast<float>((static_cast<double>(dot[j]) - m) * k - l2));
-      g = norm > 0.0 ? p - static_cast<float>(static_cast<double>(all) / norm) : 0.0f;
+      g = norm > 0.0f ? exp2f(static_cast<float>(behind)) - all / norm : 0.0f;
       if (coef != coef) g = coef;
     }
-    if (real) {
-      state[4 + 2 * j] = __float_as_int(g);
-      state[5 + 2 * j] = first ? c : -1;
-    }
+    *reinterpret_cast<int2*>(state + 4 + 2 * j) = make_int2(__float_as_int(g), first ? c : -1);
   }
-  loss = wave_sum(loss) * a.t * a.t;
-  if (lane == 0 && real) {
-    a.loss[row] = norm == 0.0 && !bad ? 0.0f : (coef != coef ? coef : static_cast<float>(loss));
+  loss = wave_add(loss) * a.t * a.t;
+  if (lane == 0) {
+    a.loss[row] = norm == 0.0f && !bad ? 0.0f : (coef != coef ? coef : loss);
     a.lse[row] = static_cast<float>(kLn2 * (l2 + m * k));
     *reinterpret_cast<v4i*>(state) = v4i{m, __float_as_int(static_cast<float>(l2)), __float_as_int(coef), 0};
   }
@@ -338,7 +377,7 @@ int forward(const char* who, const int8_t* act, long long act_pitch, const int8_
   if (const int rc = launch_vocab_stats(p.tile, l, VocabStats{part, p.tiles}, stream)) return rc;
   const VocabRows r{part, p.tiles, a.p, b.p, a.pitch, b.pitch, rows, classes, (features + 15) / 16, exp_a, exp_w, t, index, index_bytes, ignored, value, value_type,
                     top, loss, lse, state};
-  hipLaunchKernelGGL(vocab_rows_kernel, dim3((rows + 3) / 4), dim3(256), 4 * 12 * top, stream, r);
+  hipLaunchKernelGGL(vocab_rows_kernel, dim3(rows), dim3(64), 12 * top, stream, r);
   return check_launch(who);
 }
 
