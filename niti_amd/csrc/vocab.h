@@ -90,7 +90,8 @@ struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
   int weight_n;
 };
 
-enum VocabTile { kVocabLarge, kVocabMiddle, kVocabDeep, kVocabFew };
+// kinds of call by what bounds it: products (large, middle), latency (small), memory (few rows; short, up to one stage of rows)
+enum VocabTile { kVocabLarge, kVocabMiddle, kVocabSmall, kVocabShort, kVocabFew };
 VocabTile vocab_logits_tile(int rows, int classes);
 int vocab_stats_tiles(VocabTile t, int classes);    // pairs that launch_vocab_stats leaves of a row
 bool vocab_sums_wants_wide_weights(VocabTile t);

@@ -26,19 +26,21 @@ constexpr int kNone = -2147483647 - 1;                // below every logit
 enum Layout { kFast, kSlow16, kSlow8 };
 constexpr int stage_bytes(int r, Layout l) { return l == kSlow8 ? 64 * r : kStageBytes * r; }
 
-template <int TI_, int TJ_, int WI_, int WJ_, int RING_>
+template <int TI_, int TJ_, int WI_, int WJ_, int RING_, int PER_UNIT>
 struct Tile {
   static constexpr int TI = TI_, TJ = TJ_, WI = WI_, WJ = WJ_, RING = RING_;     // RING: buffers
   static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
   static constexpr int BI = TI / WI / 16, BJ = TJ / WJ / 16;   // 16 x 16 blocks of a wavefront
   static constexpr int kLds = RING * (TI + TJ) * kStageBytes;
-  // workgroups per unit that the registers are cut for: two wavefronts per SIMD at least, so that all sums are ordinary registers
-  static constexpr int kPerUnit = kWaves >= 8 ? 1 : 8 / kWaves;      // (TileDeep: one by its LDS)
+  static constexpr int kPerUnit = PER_UNIT;      // workgroups per unit that the registers are cut for
 };
-typedef Tile<256, 256, 2, 4, 2> TileLarge;
-typedef Tile<128, 128, 2, 2, 2> TileMiddle;
-typedef Tile<128, 128, 2, 2, 4> TileDeep;      // grids that leave units with one workgroup at most: what counts is how soon the loads are out
-typedef Tile<128, 32, 4, 1, 4> TileFew;
+typedef Tile<256, 256, 2, 4, 2, 1> TileLarge;
+typedef Tile<128, 128, 2, 2, 2, 2> TileMiddle;
+typedef Tile<64, 64, 2, 2, 2, 4> TileSmall;
+typedef Tile<64, 64, 2, 2, 4, 2> TileDeep;      // few tiles: what counts is how soon the loads are out
+typedef Tile<128, 32, 4, 1, 4, 2> TileFew;
+typedef Tile<128, 32, 4, 1, 3, 4> TileFewSums;
+typedef Tile<128, 128, 2, 2, 1, 4> TileShort;   // short reductions: nothing overlaps within a tile, but with three other tiles of a unit
 
 // 16-lane groups: lane i of a group names 8 bytes of a 4 x 16 block of 16-bit values (row i / 4, columns 4 (i % 4) .. + 4) and receives
 // column i of it
@@ -268,6 +270,28 @@ struct Product {
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
       for (int j = 0; j < T::BJ; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+    if constexpr (T::RING == 1) {      // a stage after the other, half after half
+      for (int s = 0; s < n; ++s) {
+        issue(0);
+        tile_sync();
+        static_for<2>([&](auto h) {
+          constexpr int SUB = decltype(h)::value;
+          static_for<T::BJ>([&](auto j) { fy.template read<SUB, decltype(j)::value>(); });
+          static_for<T::BI>([&](auto i) { fx.template read<SUB, decltype(i)::value>(); });
+          lds_settle<0>();
+          fx.template landed<SUB>();
+          fy.template landed<SUB>();
+          static_for<T::BI>([&](auto i) {
+            constexpr int I = decltype(i)::value;
+            const v4i x = fx.template get<SUB, I>();
+            static_for<T::BJ>([&](auto j) { acc[I][decltype(j)::value] = multiply(x, fy.template get<SUB, decltype(j)::value>(), acc[I][decltype(j)::value]); });
+          });
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        tile_sync();
+      }
+      return;
+    }
     // loads of the stages behind the last are issued like the others: they are out of range, and what they clear is not multiplied
     static_for<T::RING>([&](auto b) { issue(decltype(b)::value); });
     constexpr int kStageLoads = kLoadsX + kLoadsY;       // of a wavefront
@@ -321,12 +345,12 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
   int bi, bj;
   tile_of(blockIdx.x, (l.classes + T::TI - 1) / T::TI, (l.rows + T::TJ - 1) / T::TJ, &bi, &bj);
   const int i0 = bi * T::TI, j0 = bj * T::TJ;
+  const float k = exp2_scale(l);
   Product<T, kFast, kFast, v4i> p;
   p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / T::WJ, wj = wave % T::WJ;
-  const float k = exp2_scale(l);
   int2* const park = reinterpret_cast<int2*>(smem);   // [WI][TJ]
   const int v0 = i0 + wi * T::BI * 16 + 4 * (lane >> 4);
   const bool whole = i0 + T::TI <= l.classes;
@@ -425,17 +449,28 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
   int bi, bj;
   tile_of(blockIdx.x, ti, tj, &bi, &bj);
   const int i0 = bi * T::TI, j0 = bj * T::TJ;
-  Product<T, kFast, kFast, v4i> p;
-  p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave / T::WJ, wj = wave % T::WJ;
   const float k = exp2_scale(l);
+  const auto state_of = [&](int j) {
+    const int n = j0 + (wj * T::BJ + j) * 16 + (lane & 15);
+    return n < l.rows ? *reinterpret_cast<const v4i*>(g.state + n * g.state_words) : v4i{0, 0, 0, 0};
+  };
+  // the large tile has no registers to have them early
+  constexpr bool kEarly = T::TI < 256;
+  v4i early[kEarly ? T::BJ : 1];
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int j = 0; j < T::BJ; ++j) early[j] = state_of(j);
+  }
+  Product<T, kFast, kFast, v4i> p;
+  p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
   const Outgoing<T> out{smem};
 #pragma unroll
   for (int j = 0; j < T::BJ; ++j) {
     const int jt = (wj * T::BJ + j) * 16 + (lane & 15);
-    const v4i row = j0 + jt < l.rows ? *reinterpret_cast<const v4i*>(g.state + (j0 + jt) * g.state_words) : v4i{0, 0, 0, 0};
+    const v4i row = kEarly ? early[kEarly ? j : 0] : state_of(j);
     const float shift = static_cast<float>(kGradExponent) - __int_as_float(row[1]);
     const float coef = __int_as_float(row[2]);
 #pragma unroll
@@ -469,11 +504,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
   }
 }
 
-__device__ inline uint16_t bf16_of(float f) {   // round to nearest, ties to even; NaN stays NaN
-  const uint32_t u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return static_cast<uint16_t>((u >> 16) | 0x40u);
-  return static_cast<uint16_t>((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+__device__ inline uint16_t bf16_of(float f) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f)); }   // to nearest, ties to even
 
 __device__ inline int sums_exponent(const VocabSums& s) { return *s.exponent + s.bias + (s.exponent2 != nullptr ? *s.exponent2 : 0); }
 __device__ inline float sums_weight(const VocabSums& s, int j) { return s.weight == nullptr ? s.t : s.t * s.weight[s.weight_n == 1 ? 0 : j]; }
@@ -490,6 +521,7 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
   const int k0 = slice * s.steps;
   const int n = min(s.steps, stages - k0);
   const int end = min(s.nk, (k0 + n) * 64);      // steps
+  const int e = sums_exponent(s);
   Product<T, LX, LY, v4f> p;
   p.run(s.x, s.y, i0, j0, k0, n, LX == kFast ? 2 * ((end + 7) & ~7) : end, LY == kFast ? 2 * ((end + 7) & ~7) : end, smem);
   const int lane = threadIdx.x & 63;
@@ -513,7 +545,6 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
     }
     return;
   }
-  const int e = sums_exponent(s);
   const Outgoing<T> out{smem};
 #pragma unroll
   for (int j = 0; j < T::BJ; ++j) {
@@ -546,7 +577,7 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
 // large tile reads a 16-bit copy of the int8 weights: made 16-bit in registers its fragments take 487 us of 8192 x 8192 x 4096, read from
 // the copy 435, and the copy is 20 us of workgroups in the shadow of another launch.
 template <class TA, class TW>
-__global__ __launch_bounds__(TA::kThreads, TA::kPerUnit) void vocab_sums_kernel(const VocabSums a, const VocabSums w, int blocks_a) {
+__global__ __launch_bounds__(TA::kThreads, TW::kPerUnit) void vocab_sums_kernel(const VocabSums a, const VocabSums w, int blocks_a) {
   static_assert(TA::kThreads == TW::kThreads, "one launch");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   if (static_cast<int>(blockIdx.x) < blocks_a) sums_tile<TA, TA::TI == 256 ? kSlow16 : kSlow8, kFast>(a, blockIdx.x, smem);
@@ -621,7 +652,8 @@ int run_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
 }
 template <class TA, class TW>
 int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
-  constexpr int kLds = TA::kLds > TW::kLds ? TA::kLds : TW::kLds;
+  constexpr int kLdsA = TA::RING * (stage_bytes(TA::TI, TA::TI == 256 ? kSlow16 : kSlow8) + stage_bytes(TA::TJ, kFast)), kOutA = 2 * TA::TI * TA::TJ;
+  constexpr int kMostA = kLdsA > kOutA ? kLdsA : kOutA, kLds = kMostA > TW::kLds ? kMostA : TW::kLds;
   if (const int rc = with_lds<vocab_sums_kernel<TA, TW>>(kLds, "vocab_sums")) return rc;
   const long long na = (tiles_of(a.ni, a.nj, TA::TI, TA::TJ) * a.slices + 7) / 8 * 8, nw = tiles_of(w.ni, w.nj, TW::TI, TW::TJ) * w.slices;
   if (na + nw > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_sums: %lld tiles", na + nw);
@@ -634,20 +666,24 @@ int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
 // Time of a round of large tiles (one per unit) to one of middle tiles (two per unit), for equal reductions: 1.2 to 0.7.
 VocabTile vocab_logits_tile(int rows, int classes) {
   if (rows <= 32) return kVocabFew;
+  if (tiles_of(classes, rows, 64, 64) <= 512) return kVocabSmall;
   const long long middle = tiles_of(classes, rows, 128, 128);
-  if (middle <= 256) return kVocabDeep;
   const double t_large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256) * 1.2;
   const double t_middle = static_cast<double>((middle + 511) / 512) * 0.7;
   return t_large <= t_middle ? kVocabLarge : kVocabMiddle;
 }
 
-int vocab_stats_tiles(VocabTile t, int classes) { return t == kVocabLarge ? (classes + 255) / 256 : (classes + 127) / 128; }
+int vocab_stats_tiles(VocabTile t, int classes) {
+  const int classes_of_tile = t == kVocabLarge ? TileLarge::TI : (t == kVocabSmall ? TileDeep::TI : TileMiddle::TI);
+  static_assert(TileMiddle::TI == TileFew::TI, "one rule");
+  return (classes + classes_of_tile - 1) / classes_of_tile;
+}
 
 int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
   switch (t) {
     case kVocabLarge: return run_stats<TileLarge>(l, s, stream);
     case kVocabMiddle: return run_stats<TileMiddle>(l, s, stream);
-    case kVocabDeep: return run_stats<TileDeep>(l, s, stream);
+    case kVocabSmall: return run_stats<TileDeep>(l, s, stream);
     default: return run_stats<TileFew>(l, s, stream);
   }
 }
@@ -661,20 +697,28 @@ int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hip
   switch (t) {
     case kVocabLarge: return run_grad<TileLarge>(l, g, stream);
     case kVocabMiddle: return run_grad<TileMiddle>(l, g, stream);
-    case kVocabDeep: return run_grad<TileDeep>(l, g, stream);
+    case kVocabSmall: return run_grad<TileDeep>(l, g, stream);
     default: return run_grad<TileFew>(l, g, stream);
   }
 }
 
 VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w) {
   const long long large = tiles_of(features, rows, 256, 256) + tiles_of(features, classes, 256, 256);
-  const VocabTile t = rows <= 32 ? kVocabFew : (large >= 256 ? kVocabLarge : kVocabMiddle);
-  const long long na = t == kVocabFew ? tiles_of(features, rows, 128, 32) : (t == kVocabLarge ? tiles_of(features, rows, 256, 256) : tiles_of(features, rows, 128, 128));
-  const long long nw = t == kVocabLarge ? tiles_of(features, classes, 256, 256) : tiles_of(features, classes, 128, 128);
+  VocabTile t = kVocabLarge;
+  if (rows <= 256) t = rows <= 32 ? kVocabFew : kVocabShort;
+  else if (large < 256) t = tiles_of(features, classes, 128, 128) >= 256 ? kVocabMiddle : kVocabSmall;
+  long long na = 0, nw = 0;
+  switch (t) {
+    case kVocabLarge: na = tiles_of(features, rows, 256, 256), nw = tiles_of(features, classes, 256, 256); break;
+    case kVocabMiddle: na = tiles_of(features, rows, 128, 128), nw = tiles_of(features, classes, 128, 128); break;
+    case kVocabSmall: na = tiles_of(features, rows, 64, 64), nw = tiles_of(features, classes, 64, 64); break;
+    case kVocabShort: na = tiles_of(features, rows, 64, 64), nw = tiles_of(features, classes, 128, 128); break;
+    default: na = tiles_of(features, rows, 128, 32), nw = tiles_of(features, classes, 128, 128); break;
+  }
   const int sa = (classes + 63) / 64, sw = (rows + 63) / 64;
   // a workgroup's share of all stages, were they spread evenly: no tile is longer, none is cut below sixteen stages (adding the parts is
   // a launch of its own)
-  long long share = (na * sa + nw * sw) / (t == kVocabLarge ? 256 : 512) + 1;
+  long long share = (na * sa + nw * sw) / (t == kVocabLarge ? 256 : (t == kVocabMiddle ? 512 : 1024)) + 1;
   if (share < 16) share = 16;
   const auto cut = [share](int stages, int* slices, int* steps) {
     const long long want = (stages + share - 1) / share;
@@ -687,8 +731,13 @@ VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, in
 }
 
 int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream) {
-  return t == kVocabFew ? run_sums<TileFew, TileMiddle>(a, w, stream)
-                        : (t == kVocabLarge ? run_sums<TileLarge, TileLarge>(a, w, stream) : run_sums<TileMiddle, TileMiddle>(a, w, stream));
+  switch (t) {
+    case kVocabLarge: return run_sums<TileLarge, TileLarge>(a, w, stream);
+    case kVocabMiddle: return run_sums<TileMiddle, TileMiddle>(a, w, stream);
+    case kVocabSmall: return run_sums<TileSmall, TileSmall>(a, w, stream);
+    case kVocabShort: return run_sums<TileSmall, TileShort>(a, w, stream);
+    default: return run_sums<TileFewSums, TileShort>(a, w, stream);
+  }
 }
 
 int launch_vocab_join(const VocabSums* a, const VocabSums* w, hipStream_t stream) {
