@@ -50,7 +50,10 @@ int index_bytes(const at::Tensor& t, const char* who) {
   if (t.scalar_type() == at::kInt) return 4;
   refuse(std::string(who) + ": classes must be int64 or int32");
 }
-at::Tensor workspace(size_t bytes, const at::Tensor& like) { return empty8({static_cast<int64_t>(bytes > 16 ? bytes : 16)}, like); }
+// Small ones come out of the stream's own buffer, which stays; large ones go back to the allocator.
+at::Tensor workspace(size_t bytes, const at::Tensor& like) {
+  return bytes <= (32u << 20) ? scratch(bytes, like) : empty8({static_cast<int64_t>(bytes)}, like);
+}
 
 // vocab_forward(act, w, exp_a, exp_w, values or None, classes, ignored, temperature) -> (loss, lse, state)
 PyObject* forward(PyObject*, PyObject* const* args, Py_ssize_t n) {

@@ -50,6 +50,49 @@ struct VocabStats {          // (max, sum of 2^((s - max) k)) of each row over e
   int tiles;
 };
 
+// What a row learns from, and the logits there (sums of products as they are): made by workgroups of the statistics' launch
+struct VocabTargets {
+  const void* index;         // [rows][top] int32 or int64
+  int index_bytes;
+  int distill;               // 0: entropy
+  long long ignored;         // entropy: this class is none; distillation: every negative one
+  int top;
+  int32_t* state;            // receives a place's logit where its gradient will be; what an unused place receives means nothing
+};
+// class of a place: -1 none, -2 outside of the classes
+__device__ inline int vocab_target(const VocabTargets& t, long long at, int classes) {
+  const long long c = t.index_bytes == 8 ? static_cast<const int64_t*>(t.index)[at] : static_cast<const int32_t*>(t.index)[at];
+  if (t.distill ? c < 0 : c == t.ignored) return -1;
+  return c >= 0 && c < classes ? static_cast<int>(c) : -2;
+}
+
+// Sums and maxima over the wavefront by data-parallel moves (a scan inside each row of sixteen lanes, the row totals carried on), in every
+// lane: six moves of a few clocks where a shuffle through LDS is some hundred.
+template <int CTRL, int MASK>
+__device__ inline int dpp_take(int neutral, int v) { return __builtin_amdgcn_update_dpp(neutral, v, CTRL, MASK, 0xf, false); }
+template <class F>
+__device__ inline int wave_fold(int neutral, int v, F f) {
+  v = f(v, dpp_take<0x111, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x112, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x114, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x118, 0xf>(neutral, v));
+  v = f(v, dpp_take<0x142, 0xa>(neutral, v));
+  v = f(v, dpp_take<0x143, 0xc>(neutral, v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ inline int wave_add(int v) {
+  return wave_fold(0, v, [](int a, int b) { return a + b; });
+}
+__device__ inline int wave_most(int v) {
+  return wave_fold(-2147483647 - 1, v, [](int a, int b) { return max(a, b); });
+}
+__device__ inline float wave_add(float v) {
+  return __int_as_float(wave_fold(0, __float_as_int(v), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
+}
+__device__ inline float wave_most(float v) {
+  return __int_as_float(wave_fold(__float_as_int(-INFINITY), __float_as_int(v), [](int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }));
+}
+
 // int8 rows to 16-bit floats, each times weight / 2^*exponent 2^kRowExponent where there are weights; *exponent receives the smallest power of
 // two above every weight
 struct VocabWiden {
@@ -96,7 +139,7 @@ VocabTile vocab_logits_tile(int rows, int classes);
 int vocab_stats_tiles(VocabTile t, int classes);    // pairs that launch_vocab_stats leaves of a row
 bool vocab_sums_wants_wide_weights(VocabTile t);
 bool vocab_grad_writes_targets(VocabTile t, int top);
-int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream);
+int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, const VocabTargets& targets, hipStream_t stream);
 int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hipStream_t stream);
 // Both gradients' sums of a piece: a = the activations' (x: weights, int8 or a 16-bit copy, reduction slow; y: the piece's gradient, reduction fast), w = the
 // weights' (x: 16-bit activations, y: the piece's gradient, reduction slow in both)

@@ -40,6 +40,8 @@ typedef Tile<64, 64, 2, 2, 2, 4> TileSmall;
 typedef Tile<64, 64, 2, 2, 4, 2> TileDeep;      // few tiles: what counts is how soon the loads are out
 typedef Tile<128, 32, 4, 1, 4, 2> TileFew;
 typedef Tile<128, 32, 4, 1, 3, 4> TileFewSums;
+typedef Tile<128, 32, 4, 1, 8, 4> TileFewDeep;   // (one or two by its LDS)
+typedef Tile<64, 64, 2, 2, 8, 4> TileSmallDeep;
 typedef Tile<128, 128, 2, 2, 1, 4> TileShort;   // short reductions: nothing overlaps within a tile, but with three other tiles of a unit
 
 // 16-lane groups: lane i of a group names 8 bytes of a 4 x 16 block of 16-bit values (row i / 4, columns 4 (i % 4) .. + 4) and receives
@@ -339,11 +341,69 @@ __device__ inline float exp2_scale(const VocabLogits& l) {
   return fminf(k, 3.402823466e38f);
 }
 
+// folds the values of the lanes i, i ^ 16, i ^ 32, i ^ 48, which hold one column's rows
+template <class F>
+__device__ inline int fold_quarters(int v, F f) {
+  const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = f(static_cast<int>(a[0]), static_cast<int>(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return f(static_cast<int>(b[0]), static_cast<int>(b[1]));
+}
+
+constexpr int kPlaces = 8;     // of a row, whose products a wavefront makes at a time
+
+// Logits of the targets: a wavefront takes eight places of a row, its lanes sixteen features each, the loads of all in flight together.
+__device__ inline void dots_block(const VocabLogits& l, const VocabTargets& t, int block, int waves) {
+  const int lane = threadIdx.x & 63;
+  const int groups = (t.top + kPlaces - 1) / kPlaces;
+  const long long unit = static_cast<long long>(block) * waves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long row = unit / groups;
+  if (row >= l.rows) return;
+  const int j0 = static_cast<int>(unit - row * groups) * kPlaces;
+  const v4i* const arow = reinterpret_cast<const v4i*>(static_cast<const char*>(l.a.p) + row * l.a.pitch);
+  const int pieces = l.a.row_bytes / 16;
+  // a lane per place asks for its class
+  const int mine = lane < kPlaces && j0 + lane < t.top ? vocab_target(t, row * t.top + j0 + lane, l.classes) : -1;
+  v4i x = lane < pieces ? arow[lane] : v4i{0, 0, 0, 0};
+  const v4i* w[kPlaces];
+  int s[kPlaces];
+#pragma unroll
+  for (int u = 0; u < kPlaces; ++u) {
+    const int c = __builtin_amdgcn_readlane(mine, u);
+    w[u] = c < 0 ? nullptr : reinterpret_cast<const v4i*>(static_cast<const char*>(l.w.p) + c * l.w.pitch);
+    s[u] = 0;
+  }
+  for (int p = lane; p < pieces; p += 64) {
+    if (p >= 64) x = arow[p];
+    v4i y[kPlaces];
+#pragma unroll
+    for (int u = 0; u < kPlaces; ++u) y[u] = w[u] != nullptr ? w[u][p] : v4i{0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < kPlaces; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[u] = __builtin_amdgcn_sdot4(x[i], y[u][i], s[u], false);
+  }
+  int out = 0;
+#pragma unroll
+  for (int u = 0; u < kPlaces; ++u)
+    if (w[u] != nullptr) {
+      const int all = wave_add(s[u]);
+      out = lane == u ? all : out;
+    }
+  if (lane < kPlaces && j0 + lane < t.top) t.state[row * vocab_state_words(t.top) + 4 + 2 * (j0 + lane)] = out;
+}
+
+// Statistics of a tile, or - the workgroups behind the tiles - the targets' logits, which depend on nothing else either.
 template <class T>
-__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(const VocabLogits l, const VocabStats st) {
+__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(const VocabLogits l, const VocabStats st, const VocabTargets targets) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
+  if (static_cast<int>(blockIdx.x) >= ti * tj) {
+    dots_block(l, targets, blockIdx.x - ti * tj, T::kWaves);
+    return;
+  }
   int bi, bj;
-  tile_of(blockIdx.x, (l.classes + T::TI - 1) / T::TI, (l.rows + T::TJ - 1) / T::TJ, &bi, &bj);
+  tile_of(blockIdx.x, ti, tj, &bi, &bj);
   const int i0 = bi * T::TI, j0 = bj * T::TJ;
   const float k = exp2_scale(l);
   Product<T, kFast, kFast, v4i> p;
@@ -362,16 +422,14 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (whole || v0 + i * 16 + r < l.classes) m = max(m, p.acc[i][j][r]);
-    m = max(m, __shfl_xor(m, 16, 64));
-    m = max(m, __shfl_xor(m, 32, 64));
+    m = fold_quarters(m, [](int a, int b) { return max(a, b); });
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (whole || v0 + i * 16 + r < l.classes) sum += __builtin_amdgcn_exp2f(static_cast<float>(p.acc[i][j][r] - m) * k);
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
+    sum = __int_as_float(fold_quarters(__float_as_int(sum), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
     if (lane < 16) park[wi * T::TJ + (wj * T::BJ + j) * 16 + lane] = make_int2(m, __float_as_int(sum));
   }
   __syncthreads();
@@ -464,6 +522,14 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
 #pragma unroll
     for (int j = 0; j < T::BJ; ++j) early[j] = state_of(j);
   }
+  const int places = min(T::TJ, l.rows - j0) * g.top;
+  const auto place_of = [&](int at, int* j) {       // (gradient, class) of the tile's place `at`, which is row *j's
+    *j = at / max(g.top, 1);
+    return *reinterpret_cast<const int2*>(g.state + (j0 + *j) * g.state_words + 4 + 2 * (at - *j * g.top));
+  };
+  int2 place = make_int2(0, -1);
+  int place_row = 0;
+  if (kEarly && static_cast<int>(threadIdx.x) < places) place = place_of(threadIdx.x, &place_row);
   Product<T, kFast, kFast, v4i> p;
   p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
   const Outgoing<T> out{smem};
@@ -487,13 +553,11 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
   }
   __syncthreads();
   if (g.top > 0) {
-    const int rows = min(T::TJ, l.rows - j0), places = rows * g.top;
     for (int at = threadIdx.x; at < places; at += T::kThreads) {
-      const int j = at / g.top;
-      const int2 s = *reinterpret_cast<const int2*>(g.state + (j0 + j) * g.state_words + 4 + 2 * (at - j * g.top));
-      const long long i = s.y - g.first - i0;
-      if (s.y >= 0 && i >= 0 && i < T::TI && i0 + i < l.classes)
-        *out.one(j, static_cast<int>(i)) = __builtin_bit_cast(uint16_t, static_cast<_Float16>(ldexpf(__int_as_float(s.x), kGradExponent)));
+      if (!kEarly || at >= T::kThreads) place = place_of(at, &place_row);
+      const long long i = place.y - g.first - i0;
+      if (place.y >= 0 && i >= 0 && i < T::TI && i0 + i < l.classes)
+        *out.one(place_row, static_cast<int>(i)) = __builtin_bit_cast(uint16_t, static_cast<_Float16>(ldexpf(__int_as_float(place.x), kGradExponent)));
     }
     __syncthreads();
   }
@@ -635,11 +699,12 @@ int with_lds(int lds, const char* what) {   // more LDS than the default limit o
 long long tiles_of(long long ni, long long nj, int ti, int tj) { return ((ni + ti - 1) / ti) * ((nj + tj - 1) / tj); }
 
 template <class T>
-int run_stats(const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
+int run_stats(const VocabLogits& l, const VocabStats& s, const VocabTargets& targets, hipStream_t stream) {
   if (const int rc = with_lds<vocab_stats_kernel<T>>(T::kLds, "vocab_stats")) return rc;
-  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ);
-  if (tiles > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: %lld tiles", tiles);
-  hipLaunchKernelGGL(vocab_stats_kernel<T>, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, l, s);
+  const long long dots = (static_cast<long long>(l.rows) * ((targets.top + kPlaces - 1) / kPlaces) + T::kWaves - 1) / T::kWaves;
+  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ) + dots;
+  if (tiles > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: %lld workgroups", tiles);
+  hipLaunchKernelGGL(vocab_stats_kernel<T>, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, l, s, targets);
   return check_launch("vocab_stats");
 }
 template <class T>
@@ -679,12 +744,12 @@ int vocab_stats_tiles(VocabTile t, int classes) {
   return (classes + classes_of_tile - 1) / classes_of_tile;
 }
 
-int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, hipStream_t stream) {
+int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, const VocabTargets& targets, hipStream_t stream) {
   switch (t) {
-    case kVocabLarge: return run_stats<TileLarge>(l, s, stream);
-    case kVocabMiddle: return run_stats<TileMiddle>(l, s, stream);
-    case kVocabSmall: return run_stats<TileDeep>(l, s, stream);
-    default: return run_stats<TileFew>(l, s, stream);
+    case kVocabLarge: return run_stats<TileLarge>(l, s, targets, stream);
+    case kVocabMiddle: return run_stats<TileMiddle>(l, s, targets, stream);
+    case kVocabSmall: return run_stats<TileDeep>(l, s, targets, stream);
+    default: return run_stats<TileFew>(l, s, targets, stream);
   }
 }
 
@@ -716,12 +781,12 @@ VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, in
     default: na = tiles_of(features, rows, 128, 32), nw = tiles_of(features, classes, 128, 128); break;
   }
   const int sa = (classes + 63) / 64, sw = (rows + 63) / 64;
-  // a workgroup's share of all stages, were they spread evenly: no tile is longer, none is cut below sixteen stages (adding the parts is
-  // a launch of its own)
+  // a workgroup's share of all stages, were they spread evenly: no tile is longer, none is cut below eight stages, and one of up to
+  // sixteen not at all (adding the parts is a launch of its own)
   long long share = (na * sa + nw * sw) / (t == kVocabLarge ? 256 : (t == kVocabMiddle ? 512 : 1024)) + 1;
-  if (share < 16) share = 16;
+  if (share < 8) share = 8;
   const auto cut = [share](int stages, int* slices, int* steps) {
-    const long long want = (stages + share - 1) / share;
+    const long long want = stages <= 16 ? 1 : (stages + share - 1) / share;
     *steps = static_cast<int>((stages + want - 1) / want);
     *slices = (stages + *steps - 1) / *steps;
   };
@@ -731,12 +796,16 @@ VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, in
 }
 
 int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream) {
+  // Few workgroups: each of them walks along its reduction alone, at the pace of the loads that it has under way, and memory for rings of
+  // eight stages lies idle.  16 stages of 1 x 512 over 1000: 8 -> 5 us
+  const bool idle = t == kVocabFew ? tiles_of(a.ni, a.nj, 128, 32) * a.slices + tiles_of(w.ni, w.nj, 128, 128) <= 256
+                                   : tiles_of(a.ni, a.nj, 64, 64) * a.slices + tiles_of(w.ni, w.nj, 128, 128) <= 256;
   switch (t) {
     case kVocabLarge: return run_sums<TileLarge, TileLarge>(a, w, stream);
     case kVocabMiddle: return run_sums<TileMiddle, TileMiddle>(a, w, stream);
     case kVocabSmall: return run_sums<TileSmall, TileSmall>(a, w, stream);
-    case kVocabShort: return run_sums<TileSmall, TileShort>(a, w, stream);
-    default: return run_sums<TileFewSums, TileShort>(a, w, stream);
+    case kVocabShort: return idle ? run_sums<TileSmallDeep, TileShort>(a, w, stream) : run_sums<TileSmall, TileShort>(a, w, stream);
+    default: return idle ? run_sums<TileFewDeep, TileShort>(a, w, stream) : run_sums<TileFewSums, TileShort>(a, w, stream);
   }
 }
 

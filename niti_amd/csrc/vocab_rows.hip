@@ -1,7 +1,7 @@
 // Losses over a large vocabulary (vocab.h): what is done per row, the operands' layouts, and the entry points.
 //
-//   forward:  statistics of the logits per row and tile of classes (vocab.hip), then a wavefront per row joins them, multiplies out the
-//             logits of the row's targets, and leaves loss, logarithm of the denominator and what the backward pass wants to know
+//   forward:  statistics of the logits per row and tile of classes and the logits of the targets (vocab.hip), then a wavefront per row
+//             joins them and leaves loss, logarithm of the denominator and what the backward pass wants to know
 //   backward: a piece of the classes after the other: the piece's softmax as 16-bit floats (vocab.hip), the targets' places
 //             overwritten with their gradient (known in 32 bits: a small difference p - q keeps its digits), both products in one launch,
 //             their slices added in another
@@ -58,19 +58,13 @@ __global__ __launch_bounds__(256) void vocab_pad_kernel(const VocabPad a, const 
 struct VocabRows {
   const int2* part;           // [rows][tiles]
   int tiles;
-  const int8_t* a;            // 16-byte aligned rows, zero behind the features
-  const int8_t* w;
-  long long a_pitch, w_pitch;
-  int rows, classes, pieces;  // pieces of 16 features
+  int rows, classes;
   const int32_t* exp_a;
   const int32_t* exp_w;
   float t;
-  const void* index;          // [rows][top]
-  int index_bytes;
-  long long ignored;          // entropy: this class is none; distillation: every negative one
+  VocabTargets targets;
   const void* value;          // [rows][top] teacher's logits; null: entropy
   int value_type;
-  int top;
   float* loss;
   float* lse;
   int32_t* state;
@@ -82,96 +76,37 @@ __device__ inline float teacher_value(const VocabRows& a, long long i) {
   return static_cast<float>(static_cast<const _Float16*>(a.value)[i]);
 }
 
-// Sums and maxima over the wavefront by data-parallel moves (a scan inside each row of sixteen lanes, the row totals carried on), in every
-// lane: six moves of a few clocks where a shuffle through LDS is some hundred.
-template <int CTRL, int MASK>
-__device__ inline int dpp_take(int neutral, int v) { return __builtin_amdgcn_update_dpp(neutral, v, CTRL, MASK, 0xf, false); }
-template <class F>
-__device__ inline int wave_fold(int neutral, int v, F f) {
-  v = f(v, dpp_take<0x111, 0xf>(neutral, v));
-  v = f(v, dpp_take<0x112, 0xf>(neutral, v));
-  v = f(v, dpp_take<0x114, 0xf>(neutral, v));
-  v = f(v, dpp_take<0x118, 0xf>(neutral, v));
-  v = f(v, dpp_take<0x142, 0xa>(neutral, v));
-  v = f(v, dpp_take<0x143, 0xc>(neutral, v));
-  return __builtin_amdgcn_readlane(v, 63);
-}
-__device__ inline int wave_add(int v) {
-  return wave_fold(0, v, [](int a, int b) { return a + b; });
-}
-__device__ inline int wave_most(int v) {
-  return wave_fold(-2147483647 - 1, v, [](int a, int b) { return max(a, b); });
-}
-__device__ inline float wave_add(float v) {
-  return __int_as_float(wave_fold(0, __float_as_int(v), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
-}
-__device__ inline float wave_most(float v) {
-  return __int_as_float(wave_fold(__float_as_int(-INFINITY), __float_as_int(v), [](int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }));
-}
-
-// A wavefront and workgroup per row.  The loads that depend on nothing - pairs of the tiles, exponents, targets, the row's first sixteen
-// values per lane - go out together, then those of the targets' weights, eight targets at a time: what the kernel takes is the way of these.
+// A wavefront and workgroup per row.  All loads depend on nothing and go out together: pairs of the tiles, exponents, targets, their logits
+// and teacher's values; what the kernel takes is the way of these.
 __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x;
   const long long row = blockIdx.x;
+  const int top = a.targets.top;
   float* const q = reinterpret_cast<float*>(smem);
-  int* const cls = reinterpret_cast<int*>(q + a.top);
-  int* const dot = cls + a.top;
+  int* const cls = reinterpret_cast<int*>(q + top);
 
   constexpr int kHeld = 4;            // pairs in registers; a row of more tiles is read twice
   const int2* const part = a.part + row * a.tiles;
   int2 held[kHeld];
 #pragma unroll
   for (int u = 0; u < kHeld; ++u) held[u] = lane + 64 * u < a.tiles ? part[lane + 64 * u] : make_int2(-2147483647 - 1, 0);
-  const v4i* const arow = reinterpret_cast<const v4i*>(a.a + row * a.a_pitch);
-  const v4i x0 = lane < a.pieces ? arow[lane] : v4i{0, 0, 0, 0};
   const int exponent = *a.exp_a + *a.exp_w;
+  int32_t* const state = a.state + row * vocab_state_words(top);      // a place's gradient takes the place of its logit
+  const int dot0 = lane < top ? state[4 + 2 * lane] : 0;
 
   // the targets and their weights
   bool bad = false;
   float vmax = -INFINITY;
-  for (int j = lane; j < a.top; j += 64) {
-    const long long at = row * a.top + j;
-    const long long c = a.index_bytes == 8 ? static_cast<const int64_t*>(a.index)[at] : static_cast<const int32_t*>(a.index)[at];
+  for (int j = lane; j < top; j += 64) {
+    const long long at = row * top + j;
+    const int c = vocab_target(a.targets, at, a.classes);
     const float given = a.value == nullptr ? 0.0f : teacher_value(a, at) / a.t;
-    const bool none = a.value == nullptr ? c == a.ignored : c < 0;
-    if (!none && (c < 0 || c >= a.classes)) bad = true;
-    const bool used = !none && c >= 0 && c < a.classes;
-    cls[j] = used ? static_cast<int>(c) : -1;
-    const float v = used ? given : -INFINITY;
+    if (c == -2) bad = true;
+    cls[j] = c < 0 ? -1 : c;
+    const float v = c < 0 ? -INFINITY : given;
     q[j] = v;
     vmax = fmaxf(vmax, v);
-  }
-  __syncthreads();
-
-  // the targets' logits
-  for (int j0 = 0; j0 < a.top; j0 += 8) {
-    int s[8];
-    const v4i* w[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int c = j0 + u < a.top ? __builtin_amdgcn_readfirstlane(cls[j0 + u]) : -1;
-      w[u] = c < 0 ? nullptr : reinterpret_cast<const v4i*>(a.w + c * a.w_pitch);
-      s[u] = 0;
-    }
-    for (int p = lane; p < a.pieces; p += 64) {
-      const v4i x = p < 64 ? x0 : arow[p];
-      v4i y[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) y[u] = w[u] != nullptr ? w[u][p] : v4i{0, 0, 0, 0};
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[u] = __builtin_amdgcn_sdot4(x[i], y[u][i], s[u], false);
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (j0 + u < a.top) {
-        const int all = wave_add(s[u]);
-        if (lane == 0) dot[j0 + u] = all;
-      }
-    }
   }
 
   // the denominator
@@ -202,7 +137,7 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   vmax = wave_most(vmax);
   bad = __any(bad);
   float norm = 0.0f;
-  for (int j = lane; j < a.top; j += 64) {
+  for (int j = lane; j < top; j += 64) {
     const float v = q[j];
     const float e = v == -INFINITY ? 0.0f : expf(v - vmax);
     q[j] = e;
@@ -213,19 +148,18 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   __syncthreads();
 
   constexpr double kLn2 = 0.69314718055994530942;
-  int32_t* const state = a.state + row * vocab_state_words(a.top);
   float loss = 0.0f;
-  for (int j = lane; j < a.top; j += 64) {
+  for (int j = lane; j < top; j += 64) {
     const int c = cls[j];
     float g = 0.0f;
     bool first = c >= 0;
     if (c >= 0) {
       const float mine = q[j] / norm;
-      const double behind = (static_cast<double>(dot[j]) - m) * k - l2;       // log2 of the softmax here
+      const double behind = (static_cast<double>(j < 64 ? dot0 : state[4 + 2 * j]) - m) * k - l2;       // log2 of the softmax here
       if (mine > 0.0f) loss += mine * (logf(mine) - static_cast<float>(kLn2 * behind));
       else if (!(mine == 0.0f)) loss = mine;
       float all = 0.0f;                  // the weights of every place that names this class
-      for (int i = 0; i < a.top; ++i)
+      for (int i = 0; i < top; ++i)
         if (cls[i] == c) {
           all += q[i];
           if (i < j) first = false;      // one place speaks for all
@@ -374,10 +308,10 @@ int forward(const char* who, const int8_t* act, long long act_pitch, const int8_
   if (const int rc = pad_rows(&a, p.copy_a, reinterpret_cast<int8_t*>(ws + p.a), &b, p.copy_w, reinterpret_cast<int8_t*>(ws + p.w), features, stream)) return rc;
   int2* const part = reinterpret_cast<int2*>(ws + p.part);
   const VocabLogits l{bytes_operand(b, features), bytes_operand(a, features), classes, rows, features, exp_a, exp_w, 1.0f / t};
-  if (const int rc = launch_vocab_stats(p.tile, l, VocabStats{part, p.tiles}, stream)) return rc;
-  const VocabRows r{part, p.tiles, a.p, b.p, a.pitch, b.pitch, rows, classes, (features + 15) / 16, exp_a, exp_w, t, index, index_bytes, ignored, value, value_type,
-                    top, loss, lse, state};
-  hipLaunchKernelGGL(vocab_rows_kernel, dim3(rows), dim3(64), 12 * top, stream, r);
+  const VocabTargets targets{index, index_bytes, value != nullptr ? 1 : 0, ignored, top, state};
+  if (const int rc = launch_vocab_stats(p.tile, l, VocabStats{part, p.tiles}, targets, stream)) return rc;
+  const VocabRows r{part, p.tiles, rows, classes, exp_a, exp_w, t, targets, value, value_type, loss, lse, state};
+  hipLaunchKernelGGL(vocab_rows_kernel, dim3(rows), dim3(64), 8 * top, stream, r);
   return check_launch(who);
 }
 
