@@ -40,8 +40,6 @@ typedef Tile<64, 64, 2, 2, 2, 4> TileSmall;
 typedef Tile<64, 64, 2, 2, 4, 2> TileDeep;      // few tiles: what counts is how soon the loads are out
 typedef Tile<128, 32, 4, 1, 4, 2> TileFew;
 typedef Tile<128, 32, 4, 1, 3, 4> TileFewSums;
-typedef Tile<128, 32, 4, 1, 8, 4> TileFewDeep;   // (one or two by its LDS)
-typedef Tile<64, 64, 2, 2, 8, 4> TileSmallDeep;
 typedef Tile<128, 128, 2, 2, 1, 4> TileShort;   // short reductions: nothing overlaps within a tile, but with three other tiles of a unit
 
 // 16-lane groups: lane i of a group names 8 bytes of a 4 x 16 block of 16-bit values (row i / 4, columns 4 (i % 4) .. + 4) and receives
@@ -146,8 +144,9 @@ template <int R, int B, Layout L>
 struct Fragments {
   static constexpr int kAddr = L == kFast ? 2 : B;
   unsigned addr[kAddr];
-  v2i lo[2][L == kFast ? 1 : B], hi[2][L == kSlow16 ? B : 1];     // of the two halves of a stage
-  v4i whole[2][L == kFast ? B : 1];
+  // halves of a stage, of up to two stages (those that a tile does not use are no registers)
+  v2i lo[4][L == kFast ? 1 : B], hi[4][L == kSlow16 ? B : 1];
+  v4i whole[4][L == kFast ? B : 1];
 
   __device__ void init(unsigned lds, int first) {
     const int lane = threadIdx.x & 63;
@@ -167,32 +166,34 @@ struct Fragments {
 #pragma unroll
     for (int b = 0; b < kAddr; ++b) addr[b] += step;
   }
-  template <int SUB, int BLK>
+  // block BLK of half H % 2 into register set H
+  template <int H, int BLK>
   __device__ void read() {
+    constexpr int SUB = H & 1;
     if constexpr (L == kSlow16) {
-      lo[SUB][BLK] = lds_read_tr16<SUB * 64 * R>(addr[BLK]);
-      hi[SUB][BLK] = lds_read_tr16<SUB * 64 * R + 8 * R>(addr[BLK]);
+      lo[H][BLK] = lds_read_tr16<SUB * 64 * R>(addr[BLK]);
+      hi[H][BLK] = lds_read_tr16<SUB * 64 * R + 8 * R>(addr[BLK]);
     } else if constexpr (L == kSlow8) {
-      lo[SUB][BLK] = lds_read_tr8<SUB * 32 * R>(addr[BLK]);
+      lo[H][BLK] = lds_read_tr8<SUB * 32 * R>(addr[BLK]);
     } else {
-      whole[SUB][BLK] = lds_read_b128_at<BLK * 16 * kStageBytes>(addr[SUB]);
+      whole[H][BLK] = lds_read_b128_at<BLK * 16 * kStageBytes>(addr[SUB]);
     }
   }
-  // behind a settle: the reads of half SUB are in their registers
-  template <int SUB>
+  // behind a settle: the reads of set H are in their registers
+  template <int H>
   __device__ void landed() {
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      if constexpr (L == kSlow16) asm volatile("" : "+v"(lo[SUB][b]), "+v"(hi[SUB][b]));
-      else if constexpr (L == kSlow8) asm volatile("" : "+v"(lo[SUB][b]));
-      else asm volatile("" : "+v"(whole[SUB][b]));
+      if constexpr (L == kSlow16) asm volatile("" : "+v"(lo[H][b]), "+v"(hi[H][b]));
+      else if constexpr (L == kSlow8) asm volatile("" : "+v"(lo[H][b]));
+      else asm volatile("" : "+v"(whole[H][b]));
     }
   }
-  template <int SUB, int BLK>
+  template <int H, int BLK>
   __device__ v4i get() const {
-    if constexpr (L == kSlow16) return v4i{lo[SUB][BLK][0], lo[SUB][BLK][1], hi[SUB][BLK][0], hi[SUB][BLK][1]};
-    else if constexpr (L == kSlow8) return widen8(lo[SUB][BLK]);
-    else return whole[SUB][BLK];
+    if constexpr (L == kSlow16) return v4i{lo[H][BLK][0], lo[H][BLK][1], hi[H][BLK][0], hi[H][BLK][1]};
+    else if constexpr (L == kSlow8) return widen8(lo[H][BLK]);
+    else return whole[H][BLK];
   }
 };
 
@@ -259,6 +260,52 @@ struct Product {
     fy.template landed<NEXT>();
   }
 
+  // all reads / products of register set H
+  template <int H>
+  __device__ void read_all() {
+    static_for<T::BJ>([&](auto j) { fy.template read<H, decltype(j)::value>(); });
+    static_for<T::BI>([&](auto i) { fx.template read<H, decltype(i)::value>(); });
+  }
+  template <int H>
+  __device__ void landed() {
+    fx.template landed<H>();
+    fy.template landed<H>();
+  }
+  template <int H>
+  __device__ void multiply_all() {
+    static_for<T::BI>([&](auto i) {
+      constexpr int I = decltype(i)::value;
+      const v4i x = fx.template get<H, I>();
+      static_for<T::BJ>([&](auto j) { acc[I][decltype(j)::value] = multiply(x, fy.template get<H, decltype(j)::value>(), acc[I][decltype(j)::value]); });
+    });
+  }
+  // at most N of a wavefront's loads are still under way, for all wavefronts
+  template <int N>
+  __device__ void stage_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+  // A whole stage of a small tile, whose fragments are in sets 2 A and 2 A + 1: a half's few products would not cover the way of the other
+  // half's fragments, so those of the next stage are all requested ahead of this one's products.
+  template <int A>
+  __device__ void whole_stage(int& buf) {
+    constexpr int B = 1 - A;
+    stage_barrier<(T::RING - 2) * (kLoadsX + kLoadsY)>();      // the next stage has landed; this one's fragments are with every wavefront
+    const int step = buf + 1 < T::RING ? 1 : 1 - T::RING;
+    fx.other_buffer(step * kStageX);
+    fy.other_buffer(step * kStageY);
+    read_all<2 * B>();
+    read_all<2 * B + 1>();
+    issue(buf);
+    buf += step;
+    multiply_all<2 * A>();
+    multiply_all<2 * A + 1>();
+    lds_settle<0>();
+    landed<2 * B>();
+    landed<2 * B + 1>();
+  }
+
   // x, y: operands; i0, j0: the tile's corner; range of the reduction: stages k0 .. k0 + n, ending at x_end and y_end (bytes or steps)
   __device__ void run(const VocabOperand& x, const VocabOperand& y, int i0, int j0, int k0, int n, int x_end, int y_end, char* smem) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -277,17 +324,11 @@ struct Product {
         issue(0);
         tile_sync();
         static_for<2>([&](auto h) {
-          constexpr int SUB = decltype(h)::value;
-          static_for<T::BJ>([&](auto j) { fy.template read<SUB, decltype(j)::value>(); });
-          static_for<T::BI>([&](auto i) { fx.template read<SUB, decltype(i)::value>(); });
+          constexpr int H = decltype(h)::value;
+          read_all<H>();
           lds_settle<0>();
-          fx.template landed<SUB>();
-          fy.template landed<SUB>();
-          static_for<T::BI>([&](auto i) {
-            constexpr int I = decltype(i)::value;
-            const v4i x = fx.template get<SUB, I>();
-            static_for<T::BJ>([&](auto j) { acc[I][decltype(j)::value] = multiply(x, fy.template get<SUB, decltype(j)::value>(), acc[I][decltype(j)::value]); });
-          });
+          landed<H>();
+          multiply_all<H>();
           __builtin_amdgcn_sched_barrier(0);
         });
         tile_sync();
@@ -297,26 +338,28 @@ struct Product {
     // loads of the stages behind the last are issued like the others: they are out of range, and what they clear is not multiplied
     static_for<T::RING>([&](auto b) { issue(decltype(b)::value); });
     constexpr int kStageLoads = kLoadsX + kLoadsY;       // of a wavefront
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::RING - 1) * kStageLoads) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    static_for<T::BJ>([&](auto j) { fy.template read<0, decltype(j)::value>(); });
-    static_for<T::BI>([&](auto i) { fx.template read<0, decltype(i)::value>(); });
+    stage_barrier<(T::RING - 1) * kStageLoads>();
+    read_all<0>();
+    if constexpr (T::BI * T::BJ <= 4) read_all<1>();
     lds_settle<0>();
-    fx.template landed<0>();
-    fy.template landed<0>();
+    landed<0>();
     int buf = 0;
-    for (int s = 0; s < n; ++s) {
-      half<0, 1, false>(buf);
-      // the next stage has landed, and this one's buffer has been read by every wavefront
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((T::RING - 2) * kStageLoads) : "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      const int step = buf + 1 < T::RING ? 1 : 1 - T::RING;
-      fx.other_buffer(step * kStageX);
-      fy.other_buffer(step * kStageY);
-      half<1, 0, true>(buf);
-      buf += step;
+    if constexpr (T::BI * T::BJ <= 4) {
+      landed<1>();
+      for (int s = 0; s < n; s += 2) {
+        whole_stage<0>(buf);
+        if (s + 1 < n) whole_stage<1>(buf);
+      }
+    } else {
+      for (int s = 0; s < n; ++s) {
+        half<0, 1, false>(buf);
+        stage_barrier<(T::RING - 2) * kStageLoads>();      // the next stage has landed, and this one's buffer has been read by every wavefront
+        const int step = buf + 1 < T::RING ? 1 : 1 - T::RING;
+        fx.other_buffer(step * kStageX);
+        fy.other_buffer(step * kStageY);
+        half<1, 0, true>(buf);
+        buf += step;
+      }
     }
     tile_sync();            // the buffers are free
   }
@@ -796,16 +839,12 @@ VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, in
 }
 
 int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream) {
-  // Few workgroups: each of them walks along its reduction alone, at the pace of the loads that it has under way, and memory for rings of
-  // eight stages lies idle.  16 stages of 1 x 512 over 1000: 8 -> 5 us
-  const bool idle = t == kVocabFew ? tiles_of(a.ni, a.nj, 128, 32) * a.slices + tiles_of(w.ni, w.nj, 128, 128) <= 256
-                                   : tiles_of(a.ni, a.nj, 64, 64) * a.slices + tiles_of(w.ni, w.nj, 128, 128) <= 256;
   switch (t) {
     case kVocabLarge: return run_sums<TileLarge, TileLarge>(a, w, stream);
     case kVocabMiddle: return run_sums<TileMiddle, TileMiddle>(a, w, stream);
     case kVocabSmall: return run_sums<TileSmall, TileSmall>(a, w, stream);
-    case kVocabShort: return idle ? run_sums<TileSmallDeep, TileShort>(a, w, stream) : run_sums<TileSmall, TileShort>(a, w, stream);
-    default: return idle ? run_sums<TileFewDeep, TileShort>(a, w, stream) : run_sums<TileFewSums, TileShort>(a, w, stream);
+    case kVocabShort: return run_sums<TileSmall, TileShort>(a, w, stream);
+    default: return run_sums<TileFewSums, TileShort>(a, w, stream);
   }
 }
 
