@@ -33,6 +33,8 @@ struct Tile {
   static constexpr int BI = TI / WI / 16, BJ = TJ / WJ / 16;   // 16 x 16 blocks of a wavefront
   static constexpr int kLds = RING * (TI + TJ) * kStageBytes;
   static constexpr int kPerUnit = PER_UNIT;      // workgroups per unit that the registers are cut for
+  static constexpr bool kInTurn = TI == 256;     // logits: a workgroup takes several tiles in turn, with LDS for their ends behind the ring
+  static constexpr int kLdsLogits = kLds + (kInTurn ? 2 * TI * 16 * WJ : 0);
 };
 typedef Tile<256, 256, 2, 4, 2, 1> TileLarge;
 typedef Tile<128, 128, 2, 2, 2, 2> TileMiddle;
@@ -94,25 +96,10 @@ struct Source {
   // eight steps apart; kSlow8: eight of each)
   static __device__ int turn(int k) { return (L == kSlow16 ? (k & 3) | (((k >> 3) & 1) << 2) : k & 15) & (R / 16 - 1); }
 
-  // first: first row (fast) or column (slow) of the tile; k0: first stage; k_end: end of the reduction's range in bytes (fast) or steps (slow)
-  __device__ void init(const VocabOperand& o, int first, int k0, int k_end) {
+  __device__ void lanes(const VocabOperand& o) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const char* const p = static_cast<const char*>(o.p);
-    if (kSlow) {
-      const long long skip = static_cast<long long>(k0) * 64 * o.pitch + (L == kSlow16 ? 2LL : 1LL) * first;
-      base = p + skip;
-      left = (k_end - 1) * o.pitch + o.row_bytes - skip;
-      advance = 64 * o.pitch;
-      fast_left = 0;
-      piece = 0;
-    } else {
-      const long long skip = first * o.pitch + static_cast<long long>(k0) * kStageBytes;
-      base = p + skip;
-      left = (o.rows - 1) * o.pitch + o.row_bytes - skip;
-      advance = kStageBytes;
-      fast_left = k_end - k0 * kStageBytes;
-    }
+    piece = 0;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
       const int row = (q * kWaves + wave) * kRowsPerLoad + lane / kPieces;
@@ -120,6 +107,23 @@ struct Source {
       const int c = L == kFast ? slot ^ ((row >> 1) & 7) : (L == kSlow16 ? slot ^ (2 * turn(row)) : slot ^ turn(row));
       if (!kSlow) piece = c * 16;       // the same for every q: a load's rows are a multiple of 16 apart
       voff[q] = static_cast<int>(row * o.pitch) + c * 16;
+    }
+  }
+  // first: first row (fast) or column (slow) of the tile; k0: first stage; k_end: end of the reduction's range in bytes (fast) or steps (slow)
+  __device__ void seek(const VocabOperand& o, int first, int k0, int k_end) {
+    const char* const p = static_cast<const char*>(o.p);
+    if (kSlow) {
+      const long long skip = static_cast<long long>(k0) * 64 * o.pitch + (L == kSlow16 ? 2LL : 1LL) * first;
+      base = p + skip;
+      left = (k_end - 1) * o.pitch + o.row_bytes - skip;
+      advance = 64 * o.pitch;
+      fast_left = 0;
+    } else {
+      const long long skip = first * o.pitch + static_cast<long long>(k0) * kStageBytes;
+      base = p + skip;
+      left = (o.rows - 1) * o.pitch + o.row_bytes - skip;
+      advance = kStageBytes;
+      fast_left = k_end - k0 * kStageBytes;
     }
   }
 
@@ -306,19 +310,28 @@ struct Product {
     landed<2 * B + 1>();
   }
 
-  // x, y: operands; i0, j0: the tile's corner; range of the reduction: stages k0 .. k0 + n, ending at x_end and y_end (bytes or steps)
-  __device__ void run(const VocabOperand& x, const VocabOperand& y, int i0, int j0, int k0, int n, int x_end, int y_end, char* smem) {
+  __device__ void lanes(const VocabOperand& x, const VocabOperand& y, char* smem) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     ldsx = lds_addr(smem);
     ldsy = ldsx + T::RING * kStageX;
-    sx.init(x, i0, k0, x_end);
-    sy.init(y, j0, k0, y_end);
+    sx.lanes(x);
+    sy.lanes(y);
     fx.init(ldsx, (wave / T::WJ) * T::BI);
     fy.init(ldsy, (wave % T::WJ) * T::BJ);
+  }
+  __device__ void clear() {
 #pragma unroll
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
       for (int j = 0; j < T::BJ; ++j) acc[i][j] = Acc{0, 0, 0, 0};
+  }
+
+  // x, y: operands; i0, j0: the tile's corner; range of the reduction: stages k0 .. k0 + n, ending at x_end and y_end (bytes or steps)
+  __device__ void run(const VocabOperand& x, const VocabOperand& y, int i0, int j0, int k0, int n, int x_end, int y_end, char* smem) {
+    lanes(x, y, smem);
+    sx.seek(x, i0, k0, x_end);
+    sy.seek(y, j0, k0, y_end);
+    clear();
     if constexpr (T::RING == 1) {      // a stage after the other, half after half
       for (int s = 0; s < n; ++s) {
         issue(0);
@@ -376,6 +389,66 @@ __device__ inline void tile_of(int block, int ti, int tj, int* i, int* j) {
   const int rows = ti - band * kRows < kRows ? ti - band * kRows : kRows;
   *j = r / rows;
   *i = band * kRows + r - *j * rows;
+}
+
+// Logits of the tiles first, first + step, ... of `total` in turn: the last stages of a tile already load the first ones of the next, so
+// between two tiles there is only what `done` does with the first one's sums.  done(sums, i0, j0) waits for the loads under way
+// (s_waitcnt vmcnt(0)) in front of its first store - the next barrier then need not wait for its stores - and ends with a barrier if it uses LDS,
+// which is its own behind the ring.
+template <class T, class F>
+__device__ inline void logit_tiles(const VocabLogits& l, int first, int step, int total, int ti, int tj, char* smem, F done) {
+  Product<T, kFast, kFast, v4i> p;
+  static_assert(T::RING == 2 && T::BI * T::BJ > 4, "the two loads ahead of the loop; the loop of half stages");
+  const int n = (l.features + kStageBytes - 1) / kStageBytes;
+  int load_tile = first, load_stage = 0;
+  const auto seek = [&] {
+    int bi = 0, bj = 0;
+    if (load_tile < total) tile_of(load_tile, ti, tj, &bi, &bj);
+    p.sx.seek(l.w, bi * T::TI, 0, l.w.row_bytes);
+    p.sy.seek(l.a, bj * T::TJ, 0, l.a.row_bytes);
+    if (load_tile >= total) p.sx.left = p.sy.left = 0;      // nothing behind the last tile
+  };
+  const auto loaded = [&] {
+    if (++load_stage == n) {
+      load_stage = 0;
+      load_tile += step;
+      seek();
+    }
+  };
+  p.lanes(l.w, l.a, smem);
+  seek();
+  p.issue(0);
+  loaded();
+  p.issue(1);
+  loaded();
+  p.template stage_barrier<Product<T, kFast, kFast, v4i>::kLoadsX + Product<T, kFast, kFast, v4i>::kLoadsY>();
+  int buf = 0;
+  for (int tile = first; tile < total; tile += step) {
+    p.clear();
+    p.template read_all<0>();
+    lds_settle<0>();
+    p.template landed<0>();
+    for (int s = 0; s < n; ++s) {
+      p.template half<0, 1, false>(buf);
+      if (s == 0 && tile != first) {      // everything but the last tile's stores has been waited for
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      } else {
+        p.template stage_barrier<0>();
+      }
+      const int turn = buf == 0 ? 1 : -1;
+      p.fx.other_buffer(turn * p.kStageX);
+      p.fy.other_buffer(turn * p.kStageY);
+      p.template half<1, 0, true>(buf);
+      loaded();
+      buf ^= 1;
+    }
+    int bi, bj;
+    tile_of(tile, ti, tj, &bi, &bj);
+    done(p.acc, bi * T::TI, bj * T::TJ, bi);
+  }
+  tile_sync();
 }
 
 // k of vocab.h, finite: an overflow would make 0 k a NaN where it stands for a difference of nothing
@@ -436,25 +509,19 @@ __device__ inline void dots_block(const VocabLogits& l, const VocabTargets& t, i
   if (lane < kPlaces && j0 + lane < t.top) t.state[row * vocab_state_words(t.top) + 4 + 2 * (j0 + lane)] = out;
 }
 
-// Statistics of a tile, or - the workgroups behind the tiles - the targets' logits, which depend on nothing else either.
+// The thread's index, anew: what is computed from it is not kept in registers through the main loop in front.
+__device__ inline int thread_anew() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// Statistics of a tile's sums.  `park`: [WI][TJ] pairs
 template <class T>
-__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(const VocabLogits l, const VocabStats st, const VocabTargets targets) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
-  if (static_cast<int>(blockIdx.x) >= ti * tj) {
-    dots_block(l, targets, blockIdx.x - ti * tj, T::kWaves);
-    return;
-  }
-  int bi, bj;
-  tile_of(blockIdx.x, ti, tj, &bi, &bj);
-  const int i0 = bi * T::TI, j0 = bj * T::TJ;
-  const float k = exp2_scale(l);
-  Product<T, kFast, kFast, v4i> p;
-  p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ inline void stats_of(const VocabLogits& l, const VocabStats& st, const v4i (&acc)[T::BI][T::BJ], float k, int i0, int j0, int bi, int2* park) {
+  const int thread = thread_anew(), lane = thread & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
   const int wi = wave / T::WJ, wj = wave % T::WJ;
-  int2* const park = reinterpret_cast<int2*>(smem);   // [WI][TJ]
   const int v0 = i0 + wi * T::BI * 16 + 4 * (lane >> 4);
   const bool whole = i0 + T::TI <= l.classes;
 #pragma unroll
@@ -464,19 +531,19 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (whole || v0 + i * 16 + r < l.classes) m = max(m, p.acc[i][j][r]);
+        if (whole || v0 + i * 16 + r < l.classes) m = max(m, acc[i][j][r]);
     m = fold_quarters(m, [](int a, int b) { return max(a, b); });
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < T::BI; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (whole || v0 + i * 16 + r < l.classes) sum += __builtin_amdgcn_exp2f(static_cast<float>(p.acc[i][j][r] - m) * k);
+        if (whole || v0 + i * 16 + r < l.classes) sum += __builtin_amdgcn_exp2f(static_cast<float>(acc[i][j][r] - m) * k);
     sum = __int_as_float(fold_quarters(__float_as_int(sum), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
     if (lane < 16) park[wi * T::TJ + (wj * T::BJ + j) * 16 + lane] = make_int2(m, __float_as_int(sum));
   }
-  __syncthreads();
-  for (int j = threadIdx.x; j < T::TJ; j += T::kThreads) {
+  tile_sync();
+  for (int j = thread; j < T::TJ; j += T::kThreads) {
     if (j0 + j >= l.rows) break;
     int m = park[j].x;
 #pragma unroll
@@ -488,6 +555,33 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
       if (v.x != kNone) sum += __int_as_float(v.y) * __builtin_amdgcn_exp2f(static_cast<float>(v.x - m) * k);
     }
     st.part[static_cast<long long>(j0 + j) * st.tiles + bi] = make_int2(m, __float_as_int(sum));
+  }
+}
+
+// Statistics of the tiles, or - the first `others` workgroups, a multiple of eight - the targets' logits, which depend on nothing else
+// either.  Large tiles: each workgroup takes several in turn.
+template <class T>
+__global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(const VocabLogits l, const VocabStats st, const VocabTargets targets, int others) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  if (static_cast<int>(blockIdx.x) < others) {
+    dots_block(l, targets, blockIdx.x, T::kWaves);
+    return;
+  }
+  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
+  const int block = blockIdx.x - others;
+  const float k = exp2_scale(l);
+  if constexpr (T::kInTurn) {
+    int2* const park = reinterpret_cast<int2*>(smem + T::kLds);
+    logit_tiles<T>(l, block, gridDim.x - others, ti * tj, ti, tj, smem, [&](const v4i(&acc)[T::BI][T::BJ], int i0, int j0, int bi) {
+      stats_of<T>(l, st, acc, k, i0, j0, bi, park);
+      __syncthreads();
+    });
+  } else {
+    int bi, bj;
+    tile_of(block, ti, tj, &bi, &bj);
+    Product<T, kFast, kFast, v4i> p;
+    p.run(l.w, l.a, bi * T::TI, bj * T::TJ, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
+    stats_of<T>(l, st, p.acc, k, bi * T::TI, bj * T::TJ, bi, reinterpret_cast<int2*>(smem));
   }
 }
 
@@ -537,77 +631,111 @@ struct Outgoing {
   __device__ uint16_t* one(int j, int i) const { return reinterpret_cast<uint16_t*>(at(j, i >> 3)) + (i & 7); }
 };
 
+// sum_j q_j p 2^kGradExponent of four neighbouring classes of a row
+__device__ inline uint64_t grad_of(v4i s, v4i row, float k, int v, int classes) {
+  const float shift = static_cast<float>(kGradExponent) - __int_as_float(row[1]);
+  const float coef = __int_as_float(row[2]);
+  v4h o;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float e = __builtin_amdgcn_exp2f(fmaf(static_cast<float>(s[r] - row[0]), k, shift)) * coef;
+    o[r] = static_cast<_Float16>(v + r < classes ? e : 0.0f);
+  }
+  return __builtin_bit_cast(uint64_t, o);
+}
+__device__ inline uint16_t target_grad(int bits) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(ldexpf(__int_as_float(bits), kGradExponent))); }
+
 template <class T>
 __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(const VocabLogits l, const VocabGrad g) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
-  if (static_cast<int>(blockIdx.x) >= ti * tj) {
-    const int block = blockIdx.x - ti * tj;
+  const int others = (g.widen_a.blocks + g.widen_w.blocks + 7) / 8 * 8;
+  if (static_cast<int>(blockIdx.x) < others) {
+    const int block = blockIdx.x;
     if (block < g.widen_a.blocks) widen_block(g.widen_a, block, T::kThreads, smem);
-    else widen_block(g.widen_w, block - g.widen_a.blocks, T::kThreads, smem);
+    else if (block - g.widen_a.blocks < g.widen_w.blocks) widen_block(g.widen_w, block - g.widen_a.blocks, T::kThreads, smem);
     return;
   }
-  int bi, bj;
-  tile_of(blockIdx.x, ti, tj, &bi, &bj);
-  const int i0 = bi * T::TI, j0 = bj * T::TJ;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wi = wave / T::WJ, wj = wave % T::WJ;
+  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
   const float k = exp2_scale(l);
-  const auto state_of = [&](int j) {
-    const int n = j0 + (wj * T::BJ + j) * 16 + (lane & 15);
-    return n < l.rows ? *reinterpret_cast<const v4i*>(g.state + n * g.state_words) : v4i{0, 0, 0, 0};
-  };
-  // the large tile has no registers to have them early
-  constexpr bool kEarly = T::TI < 256;
-  v4i early[kEarly ? T::BJ : 1];
-  if constexpr (kEarly) {
+  const int padded = (l.classes + 7) & ~7;
+  if constexpr (T::kInTurn) {
+    // on its way out the tile passes in T::BJ parts of 16 rows per wavefront column through LDS of its own
+    const Outgoing<T> out{smem + T::kLds};
+    constexpr int kRows = 16 * T::WJ;
+    const auto row_of = [](int r, int part) { return (r >> 4) * (16 * T::BJ) + part * 16 + (r & 15); };
+    logit_tiles<T>(l, blockIdx.x - others, gridDim.x - others, ti * tj, ti, tj, smem, [&](const v4i(&acc)[T::BI][T::BJ], int i0, int j0, int) {
+      const int thread = thread_anew(), lane = thread & 63;
+      const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+      const int wi = wave / T::WJ, wj = wave % T::WJ;
+      v4i rows[T::BJ];
 #pragma unroll
-    for (int j = 0; j < T::BJ; ++j) early[j] = state_of(j);
-  }
-  const int places = min(T::TJ, l.rows - j0) * g.top;
-  const auto place_of = [&](int at, int* j) {       // (gradient, class) of the tile's place `at`, which is row *j's
-    *j = at / max(g.top, 1);
-    return *reinterpret_cast<const int2*>(g.state + (j0 + *j) * g.state_words + 4 + 2 * (at - *j * g.top));
-  };
-  int2 place = make_int2(0, -1);
-  int place_row = 0;
-  if (kEarly && static_cast<int>(threadIdx.x) < places) place = place_of(threadIdx.x, &place_row);
-  Product<T, kFast, kFast, v4i> p;
-  p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
-  const Outgoing<T> out{smem};
-#pragma unroll
-  for (int j = 0; j < T::BJ; ++j) {
-    const int jt = (wj * T::BJ + j) * 16 + (lane & 15);
-    const v4i row = kEarly ? early[kEarly ? j : 0] : state_of(j);
-    const float shift = static_cast<float>(kGradExponent) - __int_as_float(row[1]);
-    const float coef = __int_as_float(row[2]);
-#pragma unroll
-    for (int i = 0; i < T::BI; ++i) {
-      const int it = (wi * T::BI + i) * 16 + 4 * (lane >> 4);
-      v4h o;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(static_cast<float>(p.acc[i][j][r] - row[0]), k, shift)) * coef;
-        o[r] = static_cast<_Float16>(i0 + it + r < l.classes ? e : 0.0f);
+      for (int part = 0; part < T::BJ; ++part) {
+        const int n = j0 + row_of(wj * 16 + (lane & 15), part);
+        rows[part] = n < l.rows ? *reinterpret_cast<const v4i*>(g.state + n * g.state_words) : v4i{0, 0, 0, 0};
       }
-      out.put(jt, it, __builtin_bit_cast(uint64_t, o));
+#pragma unroll
+      for (int part = 0; part < T::BJ; ++part) {
+#pragma unroll
+        for (int i = 0; i < T::BI; ++i) {
+          const int it = (wi * T::BI + i) * 16 + 4 * (lane >> 4);
+          out.put(wj * 16 + (lane & 15), it, grad_of(acc[i][part], rows[part], k, i0 + it, l.classes));
+        }
+        __syncthreads();
+        if (part == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (see logit_tiles)
+#pragma unroll
+        for (int q = 0; q < kRows * Outgoing<T>::kPieces / T::kThreads; ++q) {
+          const int at = q * T::kThreads + thread, r = at / Outgoing<T>::kPieces, c = at % Outgoing<T>::kPieces, nr = j0 + row_of(r, part);
+          if (nr < l.rows && i0 + 8 * c < padded) *reinterpret_cast<v4i*>(g.g + nr * g.pitch + i0 + 8 * c) = *reinterpret_cast<const v4i*>(out.at(r, c));
+        }
+        __syncthreads();
+      }
+    });
+  } else {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave / T::WJ, wj = wave % T::WJ;
+    int bi, bj;
+    tile_of(blockIdx.x - others, ti, tj, &bi, &bj);
+    const int i0 = bi * T::TI, j0 = bj * T::TJ;
+    // what the end of the tile asks for goes out ahead of the products
+    v4i rows[T::BJ];
+#pragma unroll
+    for (int j = 0; j < T::BJ; ++j) {
+      const int n = j0 + (wj * T::BJ + j) * 16 + (lane & 15);
+      rows[j] = n < l.rows ? *reinterpret_cast<const v4i*>(g.state + n * g.state_words) : v4i{0, 0, 0, 0};
     }
-  }
-  __syncthreads();
-  if (g.top > 0) {
-    for (int at = threadIdx.x; at < places; at += T::kThreads) {
-      if (!kEarly || at >= T::kThreads) place = place_of(at, &place_row);
-      const long long i = place.y - g.first - i0;
-      if (place.y >= 0 && i >= 0 && i < T::TI && i0 + i < l.classes)
-        *out.one(place_row, static_cast<int>(i)) = __builtin_bit_cast(uint16_t, static_cast<_Float16>(ldexpf(__int_as_float(place.x), kGradExponent)));
+    const int places = min(T::TJ, l.rows - j0) * g.top;
+    const auto place_of = [&](int at, int* j) {       // (gradient, class) of the tile's place `at`, which is row *j's
+      *j = at / max(g.top, 1);
+      return *reinterpret_cast<const int2*>(g.state + (j0 + *j) * g.state_words + 4 + 2 * (at - *j * g.top));
+    };
+    int2 place = make_int2(0, -1);
+    int place_row = 0;
+    if (static_cast<int>(threadIdx.x) < places) place = place_of(threadIdx.x, &place_row);
+    Product<T, kFast, kFast, v4i> p;
+    p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
+    const Outgoing<T> out{smem};
+#pragma unroll
+    for (int j = 0; j < T::BJ; ++j) {
+#pragma unroll
+      for (int i = 0; i < T::BI; ++i) {
+        const int it = (wi * T::BI + i) * 16 + 4 * (lane >> 4);
+        out.put((wj * T::BJ + j) * 16 + (lane & 15), it, grad_of(p.acc[i][j], rows[j], k, i0 + it, l.classes));
+      }
     }
     __syncthreads();
-  }
-  const int padded = (l.classes + 7) & ~7;
-  for (int at = threadIdx.x; at < T::TJ * Outgoing<T>::kPieces; at += T::kThreads) {
-    const int j = at / Outgoing<T>::kPieces, c = at % Outgoing<T>::kPieces;
-    if (j0 + j < l.rows && i0 + 8 * c < padded) *reinterpret_cast<v4i*>(g.g + (j0 + j) * g.pitch + i0 + 8 * c) = *reinterpret_cast<const v4i*>(out.at(j, c));
+    if (g.top > 0) {
+      for (int at = threadIdx.x; at < places; at += T::kThreads) {
+        if (at >= T::kThreads) place = place_of(at, &place_row);
+        const long long i = place.y - g.first - i0;
+        if (place.y >= 0 && i >= 0 && i < T::TI && i0 + i < l.classes) *out.one(place_row, static_cast<int>(i)) = target_grad(place.x);
+      }
+      __syncthreads();
+    }
+    for (int at = threadIdx.x; at < T::TJ * Outgoing<T>::kPieces; at += T::kThreads) {
+      const int j = at / Outgoing<T>::kPieces, c = at % Outgoing<T>::kPieces;
+      if (j0 + j < l.rows && i0 + 8 * c < padded) *reinterpret_cast<v4i*>(g.g + (j0 + j) * g.pitch + i0 + 8 * c) = *reinterpret_cast<const v4i*>(out.at(j, c));
+    }
   }
 }
 
@@ -741,21 +869,27 @@ int with_lds(int lds, const char* what) {   // more LDS than the default limit o
 
 long long tiles_of(long long ni, long long nj, int ti, int tj) { return ((ni + ti - 1) / ti) * ((nj + tj - 1) / tj); }
 
+// workgroups of a logits' launch: one per tile, or as many as the device holds at once
+template <class T>
+long long logit_blocks(const VocabLogits& l) {
+  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ), units = compute_units() / 8 * 8;
+  return T::kInTurn && tiles > units ? units : tiles;
+}
 template <class T>
 int run_stats(const VocabLogits& l, const VocabStats& s, const VocabTargets& targets, hipStream_t stream) {
-  if (const int rc = with_lds<vocab_stats_kernel<T>>(T::kLds, "vocab_stats")) return rc;
-  const long long dots = (static_cast<long long>(l.rows) * ((targets.top + kPlaces - 1) / kPlaces) + T::kWaves - 1) / T::kWaves;
-  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ) + dots;
-  if (tiles > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: %lld workgroups", tiles);
-  hipLaunchKernelGGL(vocab_stats_kernel<T>, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, l, s, targets);
+  if (const int rc = with_lds<vocab_stats_kernel<T>>(T::kLdsLogits, "vocab_stats")) return rc;
+  const long long dots = ((static_cast<long long>(l.rows) * ((targets.top + kPlaces - 1) / kPlaces) + T::kWaves - 1) / T::kWaves + 7) / 8 * 8;
+  const long long blocks = logit_blocks<T>(l) + dots;
+  if (blocks > 0x7fffffffLL || tiles_of(l.classes, l.rows, T::TI, T::TJ) > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: %lld workgroups", blocks);
+  hipLaunchKernelGGL(vocab_stats_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(T::kThreads), T::kLdsLogits, stream, l, s, targets, static_cast<int>(dots));
   return check_launch("vocab_stats");
 }
 template <class T>
 int run_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
-  if (const int rc = with_lds<vocab_grad_kernel<T>>(T::kLds, "vocab_grad")) return rc;
-  const long long tiles = tiles_of(l.classes, l.rows, T::TI, T::TJ) + g.widen_a.blocks + g.widen_w.blocks;
-  if (tiles > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_grad: %lld tiles", tiles);
-  hipLaunchKernelGGL(vocab_grad_kernel<T>, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), T::kLds, stream, l, g);
+  if (const int rc = with_lds<vocab_grad_kernel<T>>(T::kLdsLogits, "vocab_grad")) return rc;
+  const long long blocks = logit_blocks<T>(l) + (g.widen_a.blocks + g.widen_w.blocks + 7) / 8 * 8;
+  if (blocks > 0x7fffffffLL || tiles_of(l.classes, l.rows, T::TI, T::TJ) > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_grad: %lld workgroups", blocks);
+  hipLaunchKernelGGL(vocab_grad_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(T::kThreads), T::kLdsLogits, stream, l, g);
   return check_launch("vocab_grad");
 }
 template <class TA, class TW>
@@ -798,8 +932,8 @@ int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, c
 
 bool vocab_sums_wants_wide_weights(VocabTile t) { return t == kVocabLarge; }
 
-// a tile looks through the places of all of its rows: up to sixteen rounds of its threads
-bool vocab_grad_writes_targets(VocabTile t, int top) { return top <= (t == kVocabLarge ? 4 : (t == kVocabFew ? 128 : 32)); }
+// a tile looks through the places of all of its rows: up to sixteen rounds of its threads.  Large ones have no registers for it
+bool vocab_grad_writes_targets(VocabTile t, int top) { return t != kVocabLarge && top <= (t == kVocabFew ? 128 : 32); }
 
 int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
   switch (t) {
