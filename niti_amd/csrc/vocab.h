@@ -27,8 +27,9 @@ constexpr int kVocabTopMost = 1024;      // places of a teacher's list (one row'
 // has named it.  Rows start on 16 bytes.
 inline __host__ __device__ long long vocab_state_words(int top) { return 4 + (2LL * top + 3) / 4 * 4; }
 
-// One operand of a product tile: rows of `pitch` bytes, 16-byte aligned.
-//   reduction index fast: `rows` rows of `row_bytes` bytes (a multiple of 16)
+// One operand of a product tile: rows of `pitch` bytes, 4-byte aligned.
+//   reduction index fast: `rows` rows of `row_bytes` readable bytes; where these are no multiple of 16, sixteen bytes at a row's end hold
+//   the beginning of what follows, and the other operand is zero there
 //   reduction index slow: `rows` steps of the reduction, tile columns along the row, whose readable length is row_bytes
 struct VocabOperand {
   const void* p;
@@ -96,8 +97,9 @@ __device__ inline float wave_most(float v) {
 // int8 rows to 16-bit floats, each times weight / 2^*exponent 2^kRowExponent where there are weights; *exponent receives the smallest power of
 // two above every weight
 struct VocabWiden {
-  const int8_t* src;         // 16-byte aligned rows, zero up to the next multiple of 16 values
+  const int8_t* src;         // rows of src_bytes readable bytes, 4-byte aligned; what is made of bytes behind `values` means nothing
   long long src_pitch;
+  int src_bytes;
   _Float16* dst;
   long long pitch;
   int rows, values;

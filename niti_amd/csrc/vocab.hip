@@ -466,6 +466,13 @@ __device__ inline int fold_quarters(int v, F f) {
   return f(static_cast<int>(b[0]), static_cast<int>(b[1]));
 }
 
+// sixteen bytes of a row of which `left` are left (a multiple of four; what lies behind the row is not touched)
+__device__ inline v4i row_piece(const char* p, int left) {
+  if (left >= 16) return *reinterpret_cast<const v4i*>(p);
+  const int* const w = reinterpret_cast<const int*>(p);
+  return v4i{left > 0 ? w[0] : 0, left > 4 ? w[1] : 0, left > 8 ? w[2] : 0, 0};
+}
+
 constexpr int kPlaces = 8;     // of a row, whose products a wavefront makes at a time
 
 // Logits of the targets: a wavefront takes eight places of a row, its lanes sixteen features each, the loads of all in flight together.
@@ -481,19 +488,19 @@ __device__ inline void dots_block(const VocabLogits& l, const VocabTargets& t, i
   // a lane per place asks for its class
   const int mine = lane < kPlaces && j0 + lane < t.top ? vocab_target(t, row * t.top + j0 + lane, l.classes) : -1;
   v4i x = lane < pieces ? arow[lane] : v4i{0, 0, 0, 0};
-  const v4i* w[kPlaces];
+  const char* w[kPlaces];
   int s[kPlaces];
 #pragma unroll
   for (int u = 0; u < kPlaces; ++u) {
     const int c = __builtin_amdgcn_readlane(mine, u);
-    w[u] = c < 0 ? nullptr : reinterpret_cast<const v4i*>(static_cast<const char*>(l.w.p) + c * l.w.pitch);
+    w[u] = c < 0 ? nullptr : static_cast<const char*>(l.w.p) + c * l.w.pitch;
     s[u] = 0;
   }
   for (int p = lane; p < pieces; p += 64) {
     if (p >= 64) x = arow[p];
     v4i y[kPlaces];
 #pragma unroll
-    for (int u = 0; u < kPlaces; ++u) y[u] = w[u] != nullptr ? w[u][p] : v4i{0, 0, 0, 0};
+    for (int u = 0; u < kPlaces; ++u) y[u] = w[u] != nullptr ? row_piece(w[u] + 16 * p, l.w.row_bytes - 16 * p) : v4i{0, 0, 0, 0};
 #pragma unroll
     for (int u = 0; u < kPlaces; ++u)
 #pragma unroll
@@ -609,7 +616,7 @@ __device__ inline void widen_block(const VocabWiden& w, int block, int threads, 
       int8_t b[16];
       v4i v;
     } u;
-    u.v = *reinterpret_cast<const v4i*>(w.src + row * w.src_pitch + c);
+    u.v = row_piece(reinterpret_cast<const char*>(w.src + row * w.src_pitch + c), w.src_bytes - c);
     if (w.weight != nullptr) scale = ldexpf(w.weight[row], kRowExponent - e);
     v8h o[2];
 #pragma unroll
@@ -944,32 +951,58 @@ int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hip
   }
 }
 
+namespace {
+// What a workgroup of the sums takes, in us: per stage and beside them, with as many of its kind on the device as `slots`.  Fitted, with
+// the two terms of the parts' adding below, to the times of every tile and cut for 27 sizes (1 to 8192 rows, 64 to 4096 features, 300 to 60032
+// classes, 970 combinations): what the plan picks is at most 3 % off the best of them.
+struct SumsCost {
+  int ti, tj, slots;
+  double stage, fixed;
+};
+struct SumsCosts {
+  VocabTile tile;
+  int rows_from, rows_to;
+  SumsCost a, w;
+};
+constexpr SumsCosts kSumsCosts[] = {
+    {kVocabLarge, 33, 0x7fffffff, {256, 256, 256, 1.3, 8.0}, {256, 256, 256, 1.05, 8.4}},
+    {kVocabMiddle, 33, 0x7fffffff, {128, 128, 512, 0.85, 4.0}, {128, 128, 512, 0.85, 4.0}},
+    {kVocabSmall, 33, 0x7fffffff, {64, 64, 1024, 0.6, 3.7}, {64, 64, 1024, 0.72, 3.0}},
+    {kVocabShort, 33, 512, {64, 64, 1024, 0.59, 3.8}, {128, 128, 1024, 1.2, 6.8}},
+    {kVocabFew, 1, 32, {128, 32, 1024, 0.24, 3.0}, {128, 128, 1024, 1.0, 1.9}},
+};
+}  // namespace
+
+// The tiles and cuts whose estimated time is least: all workgroups' time over the device's slots and half of the longest one's, and the adding
+// of the parts.
 VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w) {
-  const long long large = tiles_of(features, rows, 256, 256) + tiles_of(features, classes, 256, 256);
-  VocabTile t = kVocabLarge;
-  if (rows <= 256) t = rows <= 32 ? kVocabFew : kVocabShort;
-  else if (large < 256) t = tiles_of(features, classes, 128, 128) >= 256 ? kVocabMiddle : kVocabSmall;
-  long long na = 0, nw = 0;
-  switch (t) {
-    case kVocabLarge: na = tiles_of(features, rows, 256, 256), nw = tiles_of(features, classes, 256, 256); break;
-    case kVocabMiddle: na = tiles_of(features, rows, 128, 128), nw = tiles_of(features, classes, 128, 128); break;
-    case kVocabSmall: na = tiles_of(features, rows, 64, 64), nw = tiles_of(features, classes, 64, 64); break;
-    case kVocabShort: na = tiles_of(features, rows, 64, 64), nw = tiles_of(features, classes, 128, 128); break;
-    default: na = tiles_of(features, rows, 128, 32), nw = tiles_of(features, classes, 128, 128); break;
-  }
   const int sa = (classes + 63) / 64, sw = (rows + 63) / 64;
-  // a workgroup's share of all stages, were they spread evenly: no tile is longer, none is cut below eight stages, and one of up to
-  // sixteen not at all (adding the parts is a launch of its own)
-  long long share = (na * sa + nw * sw) / (t == kVocabLarge ? 256 : (t == kVocabMiddle ? 512 : 1024)) + 1;
-  if (share < 8) share = 8;
-  const auto cut = [share](int stages, int* slices, int* steps) {
-    const long long want = stages <= 16 ? 1 : (stages + share - 1) / share;
-    *steps = static_cast<int>((stages + want - 1) / want);
-    *slices = (stages + *steps - 1) / *steps;
-  };
-  cut(sa, slices_a, steps_a);
-  cut(sw, slices_w, steps_w);
-  return t;
+  const auto join = [features](int slices, long long nj) { return slices > 1 ? 7.2 + slices * 8.0 * features * static_cast<double>(nj) / 2e6 : 0.0; };
+  VocabTile best_tile = kVocabLarge;
+  double best = -1.0;
+  for (const SumsCosts& c : kSumsCosts) {
+    if (rows < c.rows_from || rows > c.rows_to) continue;
+    const long long na = tiles_of(features, rows, c.a.ti, c.a.tj), nw = tiles_of(features, classes, c.w.ti, c.w.tj);
+    for (int ca = 1; ca == 1 || (ca <= 64 && (sa + ca - 1) / ca >= 4); ca += (ca + 1) / 2) {
+      const int step_a = (sa + ca - 1) / ca, na_cut = (sa + step_a - 1) / step_a;
+      for (int cw = 1; cw == 1 || (cw <= 64 && (sw + cw - 1) / cw >= 4); cw += (cw + 1) / 2) {
+        const int step_w = (sw + cw - 1) / cw, nw_cut = (sw + step_w - 1) / step_w;
+        const double each_a = step_a * c.a.stage + c.a.fixed, each_w = step_w * c.w.stage + c.w.fixed;
+        const double all = na * na_cut * each_a / c.a.slots + nw * nw_cut * each_w / c.w.slots, longest = each_a > each_w ? each_a : each_w;
+        const double spread = all + 0.5 * longest;
+        const double t = (spread > longest ? spread : longest) + join(na_cut, rows) + join(nw_cut, classes);
+        if (best < 0.0 || t < best) {
+          best = t;
+          best_tile = c.tile;
+          *slices_a = na_cut;
+          *steps_a = step_a;
+          *slices_w = nw_cut;
+          *steps_w = step_w;
+        }
+      }
+    }
+  }
+  return best_tile;
 }
 
 int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream) {

@@ -189,13 +189,19 @@ __global__ __launch_bounds__(256) void vocab_targets_kernel(const int32_t* __res
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
-struct Matrix {      // as the caller has it
+struct Matrix {      // as the caller has it, or a copy with rows of a multiple of 16
   const int8_t* p;
   long long pitch;
   long long rows;
+  int row_bytes;
 };
-// the products read 16 bytes at a time, whole rows of them
-bool needs_copy(const Matrix& m, int features) { return ((reinterpret_cast<uintptr_t>(m.p) | static_cast<uintptr_t>(m.pitch) | static_cast<uintptr_t>(features)) & 15) != 0; }
+// The products read 16 bytes at a time from addresses that are multiples of four.  Activations want zeros behind their features where these are no
+// multiple of 16: the weights' row ends then do not matter.
+bool off(const Matrix& m, int features, unsigned mask) {
+  return ((reinterpret_cast<uintptr_t>(m.p) | static_cast<uintptr_t>(m.pitch) | static_cast<uintptr_t>(features)) & mask) != 0;
+}
+bool copy_activations(const Matrix& m, int features) { return off(m, features, 15); }
+bool copy_weights(const Matrix& m, int features) { return off(m, features, 3); }
 
 struct Layout {
   size_t bytes = 0;
@@ -216,8 +222,8 @@ ForwardPlan forward_plan(const Matrix& a, const Matrix& w, int features) {
   ForwardPlan p{};
   Layout l;
   const long long row = round_up(features, 16);
-  p.copy_a = needs_copy(a, features);
-  p.copy_w = needs_copy(w, features);
+  p.copy_a = copy_activations(a, features);
+  p.copy_w = copy_weights(w, features);
   p.a = l.take(p.copy_a ? a.rows * row : 0);
   p.w = l.take(p.copy_w ? w.rows * row : 0);
   p.tile = vocab_logits_tile(static_cast<int>(a.rows), static_cast<int>(w.rows));
@@ -239,8 +245,8 @@ BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
   BackwardPlan p{};
   Layout l;
   const long long row = round_up(features, 16);
-  p.copy_a = needs_copy(a, features);
-  p.copy_w = needs_copy(w, features);
+  p.copy_a = copy_activations(a, features);
+  p.copy_w = copy_weights(w, features);
   p.pitch16 = row;
   p.part_pitch = round_up(features, 4);
   long long piece = kPieceGrad / a.rows;
@@ -273,12 +279,12 @@ int pad_rows(Matrix* a, bool copy_a, int8_t* to_a, Matrix* w, bool copy_w, int8_
   };
   const VocabPad pa = pad(*a, copy_a, to_a), pw = pad(*w, copy_w, to_w);
   hipLaunchKernelGGL(vocab_pad_kernel, dim3(static_cast<unsigned>(pa.blocks) + static_cast<unsigned>(pw.blocks)), dim3(256), 0, stream, pa, pw, features);
-  if (copy_a) *a = Matrix{to_a, round_up(features, 16), a->rows};
-  if (copy_w) *w = Matrix{to_w, round_up(features, 16), w->rows};
+  if (copy_a) *a = Matrix{to_a, round_up(features, 16), a->rows, static_cast<int>(round_up(features, 16))};
+  if (copy_w) *w = Matrix{to_w, round_up(features, 16), w->rows, static_cast<int>(round_up(features, 16))};
   return check_launch("vocab_pad");
 }
-VocabOperand bytes_operand(const Matrix& m, int features) {
-  return VocabOperand{m.p, m.pitch, static_cast<int>(m.rows), static_cast<int>(round_up(features, 16))};
+VocabOperand bytes_operand(const Matrix& m) {
+  return VocabOperand{m.p, m.pitch, static_cast<int>(m.rows), m.row_bytes};
 }
 
 int check_operands(const char* who, const int8_t* act, long long act_pitch, const int8_t* w, long long w_pitch, const int32_t* exp_a, const int32_t* exp_w,
@@ -300,14 +306,14 @@ int forward(const char* who, const int8_t* act, long long act_pitch, const int8_
   if (index == nullptr || loss == nullptr || lse == nullptr || state == nullptr) return fail(NITI_ERR_INVALID_ARG, "%s: null pointer", who);
   if (index_bytes != 4 && index_bytes != 8) return fail(NITI_ERR_INVALID_ARG, "%s: classes of %d bytes (4 or 8)", who, index_bytes);
   if (!aligned16(state)) return fail(NITI_ERR_INVALID_ARG, "%s: state not 16-byte aligned", who);
-  Matrix a{act, act_pitch, rows}, b{w, w_pitch, classes};
+  Matrix a{act, act_pitch, rows, features}, b{w, w_pitch, classes, features};
   const ForwardPlan p = forward_plan(a, b, features);
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
     return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
   char* const ws = static_cast<char*>(workspace);
   if (const int rc = pad_rows(&a, p.copy_a, reinterpret_cast<int8_t*>(ws + p.a), &b, p.copy_w, reinterpret_cast<int8_t*>(ws + p.w), features, stream)) return rc;
   int2* const part = reinterpret_cast<int2*>(ws + p.part);
-  const VocabLogits l{bytes_operand(b, features), bytes_operand(a, features), classes, rows, features, exp_a, exp_w, 1.0f / t};
+  const VocabLogits l{bytes_operand(b), bytes_operand(a), classes, rows, features, exp_a, exp_w, 1.0f / t};
   const VocabTargets targets{index, index_bytes, value != nullptr ? 1 : 0, ignored, top, state};
   if (const int rc = launch_vocab_stats(p.tile, l, VocabStats{part, p.tiles}, targets, stream)) return rc;
   const VocabRows r{part, p.tiles, rows, classes, exp_a, exp_w, t, targets, value, value_type, loss, lse, state};
@@ -324,12 +330,12 @@ extern "C" size_t niti_vocab_state_words(int top) { return top > 0 ? static_cast
 
 extern "C" size_t niti_vocab_forward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
   if (rows <= 0 || features <= 0 || classes <= 0) return 0;
-  return forward_plan(Matrix{act, act_pitch, rows}, Matrix{w, w_pitch, classes}, features).bytes;
+  return forward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features).bytes;
 }
 
 extern "C" size_t niti_vocab_backward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
   if (rows <= 0 || features <= 0 || classes <= 0) return 0;
-  return backward_plan(Matrix{act, act_pitch, rows}, Matrix{w, w_pitch, classes}, features).bytes;
+  return backward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features).bytes;
 }
 
 extern "C" int niti_vocab_entropy_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
@@ -362,7 +368,7 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
   if (weight != nullptr && weights != 1 && weights != rows) return fail(NITI_ERR_INVALID_ARG, "%s: %d weights for %d rows", who, weights, rows);
   if (!(temperature > 0.0f) || !isfinite(temperature)) return fail(NITI_ERR_INVALID_ARG, "%s: temperature %g", who, static_cast<double>(temperature));
   if (!aligned16(state) || !aligned16(d_act) || !aligned16(d_w)) return fail(NITI_ERR_INVALID_ARG, "%s: state or result not 16-byte aligned", who);
-  Matrix a{act, act_pitch, rows}, b{w, w_pitch, classes};
+  Matrix a{act, act_pitch, rows, features}, b{w, w_pitch, classes, features};
   const BackwardPlan p = backward_plan(a, b, features);
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
     return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
@@ -382,12 +388,12 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
 
   for (long long first = 0; first < classes; first += p.piece) {
     const int here = static_cast<int>(classes - first < p.piece ? classes - first : p.piece);
-    const Matrix piece{b.p + first * b.pitch, b.pitch, here};
-    const VocabLogits l{bytes_operand(piece, features), bytes_operand(a, features), here, rows, features, exp_a, exp_w, 1.0f / temperature};
+    const Matrix piece{b.p + first * b.pitch, b.pitch, here, b.row_bytes};
+    const VocabLogits l{bytes_operand(piece), bytes_operand(a), here, rows, features, exp_a, exp_w, 1.0f / temperature};
     const VocabTile tile = vocab_logits_tile(rows, here);
     const bool targets = vocab_grad_writes_targets(tile, top);
-    const VocabWiden widen_a{a.p, a.pitch, wide_a, p.pitch16, rows, features, each ? weight : nullptr, exponent, first == 0 ? widen_blocks(rows) : 0};
-    const VocabWiden widen_w{piece.p, piece.pitch, wide_w, p.pitch16, here, features, nullptr, nullptr, wide_weights ? widen_blocks(here) : 0};
+    const VocabWiden widen_a{a.p, a.pitch, a.row_bytes, wide_a, p.pitch16, rows, features, each ? weight : nullptr, exponent, first == 0 ? widen_blocks(rows) : 0};
+    const VocabWiden widen_w{piece.p, piece.pitch, piece.row_bytes, wide_w, p.pitch16, here, features, nullptr, nullptr, wide_weights ? widen_blocks(here) : 0};
     if (const int rc = launch_vocab_grad(tile, l, VocabGrad{state, vocab_state_words(top), targets ? top : 0, first, grad, p.piece, widen_a, widen_w}, st)) return rc;
     if (!targets) {
       const long long places = static_cast<long long>(rows) * top;
@@ -397,7 +403,7 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
 
     const int stages = (here + 63) / 64;
     VocabSums sa{wide_weights ? VocabOperand{wide_w, p.pitch16 * 2, here, static_cast<int>(p.pitch16 * 2)}
-                              : VocabOperand{piece.p, piece.pitch, here, static_cast<int>(p.pitch16)},
+                              : VocabOperand{piece.p, piece.pitch, here, piece.row_bytes},
                  VocabOperand{grad, p.piece * 2, rows, static_cast<int>(round_up(here, 8) * 2)}, features, rows, here, (stages + p.steps_a - 1) / p.steps_a, p.steps_a,
                  p.parts_a ? reinterpret_cast<float*>(ws + p.part_a) : nullptr, p.part_pitch, first > 0 ? 1 : 0, d_act, temperature, exp_w, -kGradExponent, nullptr,
                  weight, weights};
