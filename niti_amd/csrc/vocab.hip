@@ -516,6 +516,8 @@ __device__ inline void dots_block(const VocabLogits& l, const VocabTargets& t, i
   if (lane < kPlaces && j0 + lane < t.top) t.state[row * vocab_state_words(t.top) + 4 + 2 * (j0 + lane)] = out;
 }
 
+__global__ __launch_bounds__(256) void vocab_dots_kernel(const VocabLogits l, const VocabTargets t) { dots_block(l, t, blockIdx.x, 4); }
+
 // The thread's index, anew: what is computed from it is not kept in registers through the main loop in front.
 __device__ inline int thread_anew() {
   int t = threadIdx.x;
@@ -598,7 +600,14 @@ __device__ inline void widen_block(const VocabWiden& w, int block, int threads, 
   if (w.weight != nullptr) {
     float* const most = reinterpret_cast<float*>(smem);
     float m = 0.0f;
-    for (int i = threadIdx.x; i < w.rows; i += threads) m = fmaxf(m, fabsf(w.weight[i]));
+    constexpr int kAhead = 8;       // loads under way together
+    for (int i = threadIdx.x; i < w.rows; i += kAhead * threads) {
+      float v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) v[u] = i + u * threads < w.rows ? w.weight[i + u * threads] : 0.0f;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) m = fmaxf(m, fabsf(v[u]));
+    }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
@@ -610,7 +619,7 @@ __device__ inline void widen_block(const VocabWiden& w, int block, int threads, 
   const int pieces = (w.values + 15) / 16;
   const long long all = static_cast<long long>(w.rows) * pieces;
   for (long long at = static_cast<long long>(block) * threads + threadIdx.x; at < all; at += static_cast<long long>(w.blocks) * threads) {
-    const long long row = at / pieces;
+    const long long row = all < 0x7fffffffLL ? static_cast<unsigned>(at) / static_cast<unsigned>(pieces) : at / pieces;
     const int c = static_cast<int>(at - row * pieces) * 16;
     union {
       int8_t b[16];
@@ -655,14 +664,15 @@ __device__ inline uint16_t target_grad(int bits) { return __builtin_bit_cast(uin
 template <class T>
 __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(const VocabLogits l, const VocabGrad g) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
+  // the copies' workgroups (a multiple of eight) come first where the tiles' stay to the end, behind the tiles otherwise
+  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
   const int others = (g.widen_a.blocks + g.widen_w.blocks + 7) / 8 * 8;
-  if (static_cast<int>(blockIdx.x) < others) {
-    const int block = blockIdx.x;
-    if (block < g.widen_a.blocks) widen_block(g.widen_a, block, T::kThreads, smem);
-    else if (block - g.widen_a.blocks < g.widen_w.blocks) widen_block(g.widen_w, block - g.widen_a.blocks, T::kThreads, smem);
+  const int copy = T::kInTurn ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) - ti * tj;
+  if (T::kInTurn ? copy < others : copy >= 0) {
+    if (copy < g.widen_a.blocks) widen_block(g.widen_a, copy, T::kThreads, smem);
+    else if (copy - g.widen_a.blocks < g.widen_w.blocks) widen_block(g.widen_w, copy - g.widen_a.blocks, T::kThreads, smem);
     return;
   }
-  const int ti = (l.classes + T::TI - 1) / T::TI, tj = (l.rows + T::TJ - 1) / T::TJ;
   const float k = exp2_scale(l);
   const int padded = (l.classes + 7) & ~7;
   if constexpr (T::kInTurn) {
@@ -702,7 +712,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave / T::WJ, wj = wave % T::WJ;
     int bi, bj;
-    tile_of(blockIdx.x - others, ti, tj, &bi, &bj);
+    tile_of(blockIdx.x, ti, tj, &bi, &bj);
     const int i0 = bi * T::TI, j0 = bj * T::TJ;
     // what the end of the tile asks for goes out ahead of the products
     v4i rows[T::BJ];
@@ -807,10 +817,26 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
       if (j0 + j < s.nj && i0 + 8 * c < s.ni)
         *reinterpret_cast<v4i*>(s.out + static_cast<long long>(j0 + j) * s.ni + i0 + 8 * c) = *reinterpret_cast<const v4i*>(out.at(j, c));
     }
-  } else {      // rows that start anywhere: a value per lane, neighbours in neighbouring lanes
-    for (int at = threadIdx.x; at < T::TJ * T::TI; at += T::kThreads) {
-      const int j = at / T::TI, i = at % T::TI;
-      if (j0 + j < s.nj && i0 + i < s.ni) s.out[static_cast<long long>(j0 + j) * s.ni + i0 + i] = *out.one(j, i);
+  } else {      // rows that start anywhere: whole sixteen bytes from the first multiple of sixteen on, then what is left at both ends
+    const int width = min(T::TI, s.ni - i0), rows = min(T::TJ, s.nj - j0);
+    const auto row_of = [&](int j) { return s.out + static_cast<long long>(j0 + j) * s.ni + i0; };
+    const auto lead_of = [&](const uint16_t* row) { return min(width, static_cast<int>((-reinterpret_cast<intptr_t>(row) & 15) >> 1)); };
+    for (int at = threadIdx.x; at < rows * Outgoing<T>::kPieces; at += T::kThreads) {
+      const int j = at / Outgoing<T>::kPieces, c = at % Outgoing<T>::kPieces;
+      uint16_t* const row = row_of(j);
+      const int from = lead_of(row) + 8 * c;
+      if (from + 8 > width) continue;
+      v4i v;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) v[d] = *out.one(j, from + 2 * d) | *out.one(j, from + 2 * d + 1) << 16;
+      *reinterpret_cast<v4i*>(row + from) = v;
+    }
+    for (int at = threadIdx.x; at < rows * 16; at += T::kThreads) {      // up to seven values in front and behind
+      const int j = at >> 4, e = at & 15;
+      uint16_t* const row = row_of(j);
+      const int lead = lead_of(row), behind = lead + (width - lead) / 8 * 8;
+      const int i = e < 8 ? e : behind + e - 8;
+      if (e < 8 ? i < lead : i < width) row[i] = *out.one(j, i);
     }
   }
 }
@@ -829,9 +855,9 @@ __global__ __launch_bounds__(TA::kThreads, TW::kPerUnit) void vocab_sums_kernel(
 // adds the slices, scales, rounds; a lane takes four neighbours of a row
 __device__ inline void join_block(const VocabSums& s, long long block) {
   const int quads = (s.ni + 3) / 4;
-  const long long at = block * 256 + threadIdx.x;
-  if (at >= static_cast<long long>(quads) * s.nj) return;
-  const int j = static_cast<int>(at / quads), i = static_cast<int>(at - static_cast<long long>(j) * quads) * 4;
+  const long long at = block * 256 + threadIdx.x, all = static_cast<long long>(quads) * s.nj;
+  if (at >= all) return;
+  const int j = static_cast<int>(all < 0x7fffffffLL ? static_cast<unsigned>(at) / static_cast<unsigned>(quads) : at / quads), i = static_cast<int>(at - static_cast<long long>(j) * quads) * 4;
   v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
   const float* p = s.part + j * s.part_pitch + i;
   const long long slice = static_cast<long long>(s.nj) * s.part_pitch;
@@ -885,7 +911,15 @@ long long logit_blocks(const VocabLogits& l) {
 template <class T>
 int run_stats(const VocabLogits& l, const VocabStats& s, const VocabTargets& targets, hipStream_t stream) {
   if (const int rc = with_lds<vocab_stats_kernel<T>>(T::kLdsLogits, "vocab_stats")) return rc;
-  const long long dots = ((static_cast<long long>(l.rows) * ((targets.top + kPlaces - 1) / kPlaces) + T::kWaves - 1) / T::kWaves + 7) / 8 * 8;
+  // beside the tiles they have the tiles' LDS, hence few wavefronts of a unit: many go out in a launch of their own
+  const long long units = static_cast<long long>(l.rows) * ((targets.top + kPlaces - 1) / kPlaces);
+  const bool apart = units > 4096;
+  if (apart) {
+    if (units > 4LL * 0x7fffffff) return fail(NITI_ERR_UNSUPPORTED, "vocab_dots: %lld groups of places", units);
+    hipLaunchKernelGGL(vocab_dots_kernel, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, stream, l, targets);
+    if (const int rc = check_launch("vocab_dots")) return rc;
+  }
+  const long long dots = apart ? 0 : ((units + T::kWaves - 1) / T::kWaves + 7) / 8 * 8;
   const long long blocks = logit_blocks<T>(l) + dots;
   if (blocks > 0x7fffffffLL || tiles_of(l.classes, l.rows, T::TI, T::TJ) > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: %lld workgroups", blocks);
   hipLaunchKernelGGL(vocab_stats_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(T::kThreads), T::kLdsLogits, stream, l, s, targets, static_cast<int>(dots));

@@ -33,9 +33,9 @@ __global__ __launch_bounds__(256) void vocab_pad_kernel(const VocabPad a, const 
   const bool first = static_cast<int>(blockIdx.x) < a.blocks;
   const VocabPad p = first ? a : b;
   const int pieces = (n + 15) / 16;
-  const long long at = static_cast<long long>(blockIdx.x - (first ? 0 : a.blocks)) * 256 + threadIdx.x;
-  if (at >= p.rows * pieces) return;
-  const long long row = at / pieces;
+  const long long at = static_cast<long long>(blockIdx.x - (first ? 0 : a.blocks)) * 256 + threadIdx.x, all = p.rows * pieces;
+  if (at >= all) return;
+  const long long row = all < 0x7fffffffLL ? static_cast<unsigned>(at) / static_cast<unsigned>(pieces) : at / pieces;
   const int c = static_cast<int>(at - row * pieces) * 16;
   const uintptr_t from = reinterpret_cast<uintptr_t>(p.src + row * p.pitch + c);
   const uint32_t* const words = reinterpret_cast<const uint32_t*>(from & ~static_cast<uintptr_t>(3));
@@ -197,11 +197,9 @@ struct Matrix {      // as the caller has it, or a copy with rows of a multiple 
 };
 // The products read 16 bytes at a time from addresses that are multiples of four.  Activations want zeros behind their features where these are no
 // multiple of 16: the weights' row ends then do not matter.
-bool off(const Matrix& m, int features, unsigned mask) {
-  return ((reinterpret_cast<uintptr_t>(m.p) | static_cast<uintptr_t>(m.pitch) | static_cast<uintptr_t>(features)) & mask) != 0;
-}
-bool copy_activations(const Matrix& m, int features) { return off(m, features, 15); }
-bool copy_weights(const Matrix& m, int features) { return off(m, features, 3); }
+bool off_four(const Matrix& m) { return ((reinterpret_cast<uintptr_t>(m.p) | static_cast<uintptr_t>(m.pitch)) & 3) != 0; }
+bool copy_activations(const Matrix& m, int features) { return off_four(m) || features % 16 != 0; }
+bool copy_weights(const Matrix& m, int features) { return off_four(m) || features % 4 != 0; }
 
 struct Layout {
   size_t bytes = 0;
