@@ -946,14 +946,15 @@ int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
 
 }  // namespace
 
-// Time of a round of large tiles (one per unit) to one of middle tiles (two per unit), for equal reductions: 1.2 to 0.7.
+// Statistics and gradients of 48 sizes (64 to 8192 rows, 512 to 100096 classes, 64 to 2048 features) with each tile: a full round of large
+// tiles (one per unit, in turn: whole rounds) takes 1.68 times one of middle tiles (two per unit, whose rounds overlap), at 64 and
+// at 2048 features alike.  64 x 64 tiles where the device holds them all at once (64 rows of 64 features over 20032 classes: 4.4 us, middle 4.9; of 2048:
+// 11 and 16; 128 of 512 over 100096: 28 and 18).
 VocabTile vocab_logits_tile(int rows, int classes) {
   if (rows <= 32) return kVocabFew;
   if (tiles_of(classes, rows, 64, 64) <= 512) return kVocabSmall;
-  const long long middle = tiles_of(classes, rows, 128, 128);
-  const double t_large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256) * 1.2;
-  const double t_middle = static_cast<double>((middle + 511) / 512) * 0.7;
-  return t_large <= t_middle ? kVocabLarge : kVocabMiddle;
+  const double large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256), middle = static_cast<double>(tiles_of(classes, rows, 128, 128)) / 512;
+  return 1.68 * large <= middle ? kVocabLarge : kVocabMiddle;
 }
 
 int vocab_stats_tiles(VocabTile t, int classes) {
