@@ -135,9 +135,10 @@ struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
   int weight_n;
 };
 
-// kinds of call by what bounds it: products (large, middle), latency (small), memory (few rows; short, up to one stage of rows)
-enum VocabTile { kVocabLarge, kVocabMiddle, kVocabSmall, kVocabShort, kVocabFew };
-VocabTile vocab_logits_tile(int rows, int classes);
+// The tiles of a launch (vocab.hip): 256 x 256; 128 x 128 two to a unit; 64 x 64; short, the sums of few rows (64 x 64 for the activations, one
+// buffer of 128 x 128 for the weights); 32 rows; 128 x 128 in one buffer, four to a unit
+enum VocabTile { kVocabLarge, kVocabMiddle, kVocabSmall, kVocabShort, kVocabFew, kVocabQuad };
+VocabTile vocab_logits_tile(int rows, int features, int classes);
 int vocab_stats_tiles(VocabTile t, int classes);    // pairs that launch_vocab_stats leaves of a row
 bool vocab_sums_wants_wide_weights(VocabTile t);
 bool vocab_grad_writes_targets(VocabTile t, int top);

@@ -714,12 +714,16 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
     int bi, bj;
     tile_of(blockIdx.x, ti, tj, &bi, &bj);
     const int i0 = bi * T::TI, j0 = bj * T::TJ;
-    // what the end of the tile asks for goes out ahead of the products
-    v4i rows[T::BJ];
-#pragma unroll
-    for (int j = 0; j < T::BJ; ++j) {
+    // what the end of the tile asks for goes out ahead of the products, where there are registers for it
+    constexpr bool kEarly = T::RING > 1;
+    const auto state_of = [&](int j) {
       const int n = j0 + (wj * T::BJ + j) * 16 + (lane & 15);
-      rows[j] = n < l.rows ? *reinterpret_cast<const v4i*>(g.state + n * g.state_words) : v4i{0, 0, 0, 0};
+      return n < l.rows ? *reinterpret_cast<const v4i*>(g.state + n * g.state_words) : v4i{0, 0, 0, 0};
+    };
+    v4i rows[T::BJ];
+    if constexpr (kEarly) {
+#pragma unroll
+      for (int j = 0; j < T::BJ; ++j) rows[j] = state_of(j);
     }
     const int places = min(T::TJ, l.rows - j0) * g.top;
     const auto place_of = [&](int at, int* j) {       // (gradient, class) of the tile's place `at`, which is row *j's
@@ -728,10 +732,14 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
     };
     int2 place = make_int2(0, -1);
     int place_row = 0;
-    if (static_cast<int>(threadIdx.x) < places) place = place_of(threadIdx.x, &place_row);
+    if (kEarly && static_cast<int>(threadIdx.x) < places) place = place_of(threadIdx.x, &place_row);
     Product<T, kFast, kFast, v4i> p;
     p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
     const Outgoing<T> out{smem};
+    if constexpr (!kEarly) {
+#pragma unroll
+      for (int j = 0; j < T::BJ; ++j) rows[j] = state_of(j);
+    }
 #pragma unroll
     for (int j = 0; j < T::BJ; ++j) {
 #pragma unroll
@@ -743,7 +751,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
     __syncthreads();
     if (g.top > 0) {
       for (int at = threadIdx.x; at < places; at += T::kThreads) {
-        if (at >= T::kThreads) place = place_of(at, &place_row);
+        if (!kEarly || at >= T::kThreads) place = place_of(at, &place_row);
         const long long i = place.y - g.first - i0;
         if (place.y >= 0 && i >= 0 && i < T::TI && i0 + i < l.classes) *out.one(place_row, static_cast<int>(i)) = target_grad(place.x);
       }
@@ -946,15 +954,19 @@ int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
 
 }  // namespace
 
-// Statistics and gradients of 48 sizes (64 to 8192 rows, 512 to 100096 classes, 64 to 2048 features) with each tile: a full round of large
-// tiles (one per unit, in turn: whole rounds) takes 1.68 times one of middle tiles (two per unit, whose rounds overlap), at 64 and
-// at 2048 features alike.  64 x 64 tiles where the device holds them all at once (64 rows of 64 features over 20032 classes: 4.4 us, middle 4.9; of 2048:
-// 11 and 16; 128 of 512 over 100096: 28 and 18).
-VocabTile vocab_logits_tile(int rows, int classes) {
+// By statistics and gradients of 60 sizes (64 to 8192 rows, 512 to 100096 classes, 64 to 2048 features) with each tile.
+//   64 x 64 where the device holds them all at once: 64 rows of 64 features over 20032 classes 4.4 us (128 x 128 4.9), of 2048 11 (16)
+//   128 x 128 in a ring of two, two to a unit, where the device holds these at once and there are stages to overlap: 256 x 1024 over 10048 8.7
+//   (one buffer and four to a unit 11.2), 256 x 256 5.6 (5.9), 256 x 64 5.0 (4.9)
+//   256 x 256 in turn for long reductions on many rounds: a round is 1.68 of 128 x 128.  2048 x 2048 over 32064 141 (157), x 1024 79 (78), x 512 52 (48)
+//   128 x 128 in one buffer, four to a unit, elsewhere: 1024 x 64 over 100096 41 (256 x 256 55, ring of two 60), 300 x 1024 over 30016 17 (22, 20)
+VocabTile vocab_logits_tile(int rows, int features, int classes) {
   if (rows <= 32) return kVocabFew;
   if (tiles_of(classes, rows, 64, 64) <= 512) return kVocabSmall;
-  const double large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256), middle = static_cast<double>(tiles_of(classes, rows, 128, 128)) / 512;
-  return 1.68 * large <= middle ? kVocabLarge : kVocabMiddle;
+  const double middle = static_cast<double>(tiles_of(classes, rows, 128, 128)) / 512;
+  if (middle <= 1.0) return features >= 512 ? kVocabMiddle : kVocabQuad;
+  const double large = static_cast<double>((tiles_of(classes, rows, 256, 256) + 255) / 256);
+  return features > 1024 && 1.68 * large <= middle ? kVocabLarge : kVocabQuad;
 }
 
 int vocab_stats_tiles(VocabTile t, int classes) {
@@ -968,6 +980,7 @@ int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, c
     case kVocabLarge: return run_stats<TileLarge>(l, s, targets, stream);
     case kVocabMiddle: return run_stats<TileMiddle>(l, s, targets, stream);
     case kVocabSmall: return run_stats<TileDeep>(l, s, targets, stream);
+    case kVocabQuad: return run_stats<TileShort>(l, s, targets, stream);
     default: return run_stats<TileFew>(l, s, targets, stream);
   }
 }
@@ -982,14 +995,15 @@ int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hip
     case kVocabLarge: return run_grad<TileLarge>(l, g, stream);
     case kVocabMiddle: return run_grad<TileMiddle>(l, g, stream);
     case kVocabSmall: return run_grad<TileDeep>(l, g, stream);
+    case kVocabQuad: return run_grad<TileShort>(l, g, stream);
     default: return run_grad<TileFew>(l, g, stream);
   }
 }
 
 namespace {
 // What a workgroup of the sums takes, in us: per stage and beside them, with as many of its kind on the device as `slots`.  Fitted, with
-// the two terms of the parts' adding below, to the times of every tile and cut for 27 sizes (1 to 8192 rows, 64 to 4096 features, 300 to 60032
-// classes, 970 combinations): what the plan picks is at most 3 % off the best of them.
+// the two terms of the parts' adding below, to the times of every tile and cut for 35 sizes (1 to 8192 rows, 64 to 4096 features, 100 to 60032
+// classes, some 1400 combinations): what the plan picks is at most 4 % off the best of them.
 struct SumsCost {
   int ti, tj, slots;
   double stage, fixed;
@@ -1000,19 +1014,20 @@ struct SumsCosts {
   SumsCost a, w;
 };
 constexpr SumsCosts kSumsCosts[] = {
-    {kVocabLarge, 33, 0x7fffffff, {256, 256, 256, 1.3, 8.0}, {256, 256, 256, 1.05, 8.4}},
-    {kVocabMiddle, 33, 0x7fffffff, {128, 128, 512, 0.85, 4.0}, {128, 128, 512, 0.85, 4.0}},
-    {kVocabSmall, 33, 0x7fffffff, {64, 64, 1024, 0.6, 3.7}, {64, 64, 1024, 0.72, 3.0}},
-    {kVocabShort, 33, 512, {64, 64, 1024, 0.59, 3.8}, {128, 128, 1024, 1.2, 6.8}},
+    {kVocabLarge, 33, 0x7fffffff, {256, 256, 256, 1.3, 6.0}, {256, 256, 256, 1.14, 8.4}},
+    {kVocabMiddle, 33, 0x7fffffff, {128, 128, 512, 0.85, 5.5}, {128, 128, 512, 0.85, 4.0}},
+    {kVocabQuad, 33, 0x7fffffff, {128, 128, 1024, 1.4, 6.0}, {128, 128, 1024, 1.2, 6.0}},
+    {kVocabSmall, 33, 0x7fffffff, {64, 64, 1024, 0.7, 3.7}, {64, 64, 1024, 0.84, 3.0}},
+    {kVocabShort, 33, 512, {64, 64, 1024, 0.61, 2.85}, {128, 128, 1024, 1.2, 6.8}},
     {kVocabFew, 1, 32, {128, 32, 1024, 0.24, 3.0}, {128, 128, 1024, 1.0, 1.9}},
 };
 }  // namespace
 
-// The tiles and cuts whose estimated time is least: all workgroups' time over the device's slots and half of the longest one's, and the adding
+// The tiles and cuts whose estimated time is least: all workgroups' time over the device's slots and a part of the longest one's, and the adding
 // of the parts.
 VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w) {
   const int sa = (classes + 63) / 64, sw = (rows + 63) / 64;
-  const auto join = [features](int slices, long long nj) { return slices > 1 ? 7.2 + slices * 8.0 * features * static_cast<double>(nj) / 2e6 : 0.0; };
+  const auto join = [features](int slices, long long nj) { return slices > 1 ? 7.7 + slices * 8.0 * features * static_cast<double>(nj) / 2.8e6 : 0.0; };
   VocabTile best_tile = kVocabLarge;
   double best = -1.0;
   for (const SumsCosts& c : kSumsCosts) {
@@ -1024,7 +1039,7 @@ VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, in
         const int step_w = (sw + cw - 1) / cw, nw_cut = (sw + step_w - 1) / step_w;
         const double each_a = step_a * c.a.stage + c.a.fixed, each_w = step_w * c.w.stage + c.w.fixed;
         const double all = na * na_cut * each_a / c.a.slots + nw * nw_cut * each_w / c.w.slots, longest = each_a > each_w ? each_a : each_w;
-        const double spread = all + 0.5 * longest;
+        const double spread = all + 0.27 * longest;
         const double t = (spread > longest ? spread : longest) + join(na_cut, rows) + join(nw_cut, classes);
         if (best < 0.0 || t < best) {
           best = t;
@@ -1046,6 +1061,7 @@ int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipSt
     case kVocabMiddle: return run_sums<TileMiddle, TileMiddle>(a, w, stream);
     case kVocabSmall: return run_sums<TileSmall, TileSmall>(a, w, stream);
     case kVocabShort: return run_sums<TileSmall, TileShort>(a, w, stream);
+    case kVocabQuad: return run_sums<TileShort, TileShort>(a, w, stream);
     default: return run_sums<TileFewSums, TileShort>(a, w, stream);
   }
 }

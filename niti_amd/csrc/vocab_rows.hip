@@ -224,7 +224,7 @@ ForwardPlan forward_plan(const Matrix& a, const Matrix& w, int features) {
   p.copy_w = copy_weights(w, features);
   p.a = l.take(p.copy_a ? a.rows * row : 0);
   p.w = l.take(p.copy_w ? w.rows * row : 0);
-  p.tile = vocab_logits_tile(static_cast<int>(a.rows), static_cast<int>(w.rows));
+  p.tile = vocab_logits_tile(static_cast<int>(a.rows), features, static_cast<int>(w.rows));
   p.tiles = vocab_stats_tiles(p.tile, static_cast<int>(w.rows));
   p.part = l.take(a.rows * p.tiles * 8);
   p.bytes = l.bytes;
@@ -388,7 +388,7 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
     const int here = static_cast<int>(classes - first < p.piece ? classes - first : p.piece);
     const Matrix piece{b.p + first * b.pitch, b.pitch, here, b.row_bytes};
     const VocabLogits l{bytes_operand(piece), bytes_operand(a), here, rows, features, exp_a, exp_w, 1.0f / temperature};
-    const VocabTile tile = vocab_logits_tile(rows, here);
+    const VocabTile tile = vocab_logits_tile(rows, features, here);
     const bool targets = vocab_grad_writes_targets(tile, top);
     const VocabWiden widen_a{a.p, a.pitch, a.row_bytes, wide_a, p.pitch16, rows, features, each ? weight : nullptr, exponent, first == 0 ? widen_blocks(rows) : 0};
     const VocabWiden widen_w{piece.p, piece.pitch, piece.row_bytes, wide_w, p.pitch16, here, features, nullptr, nullptr, wide_weights ? widen_blocks(here) : 0};
