@@ -582,8 +582,8 @@ int niti_group_conv_i8_f32(const int8_t* x, const int8_t* w, float* y, int N, in
 /*
  * Losses over many classes, the logits kept nowhere.  No counterpart in the reference, whose loss (ti_loss.py:5-36) takes int8
  * logits that lie in memory.  act: [rows][features] int8, w: [classes][features] int8, rows act_pitch / w_pitch bytes apart (any
- * alignment; multiples of 16 bytes throughout are read in place), exponents in device memory; a logit is
- * z = (act . w) 2^(exp_a + exp_w), the sum exact in int32 (features <= 65536).
+ * alignment; read in place where address and pitch are multiples of four bytes and the features of 16, the weights' of 4), exponents in
+ * device memory; a logit is z = (act . w) 2^(exp_a + exp_w), the sum exact in int32 (features <= 65536).
  *
  * niti_vocab_entropy_i8: loss[n] = log sum_v exp(z[n,v]) - z[n,target[n]], lse[n] = log sum_v exp(z[n,v]) in float32.  target: int32
  * or int64 by target_bytes.  A row whose target is `ignored` has loss 0 and no gradient; any other target outside the classes
@@ -598,7 +598,7 @@ int niti_group_conv_i8_f32(const int8_t* x, const int8_t* w, float* y, int N, in
  * Both leave in `state` (rows * niti_vocab_state_words(top) int32, 16-byte aligned; top = 1 for the entropy) what niti_vocab_backward_i8 needs: gradients
  * of sum_n weight[n] loss[n] with respect to act 2^exp_a (d_act [rows][features]) and w 2^exp_w (d_w [classes][features]) as bfloat16, from
  * sums in float32.  weight: `weights` = rows values, one for all, or null for 1.  The logits are computed again, a piece of the
- * classes at a time; the softmax of a piece is held as float16 times 2^15.
+ * classes at a time; the softmax of a piece, times 2^15, and weight[n] act, over a power of two, are held as float16.
  *
  * The workspaces depend on the operands' addresses through their alignment alone.
  */

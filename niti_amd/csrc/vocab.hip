@@ -3,16 +3,18 @@
 //
 // Tile: TI x TJ results of sum_k x[i][k] y[j][k]; lane l of a wavefront holds for each 16 x 16 block column j = l % 16 and the rows
 // i = 4 (l / 16) .. + 4 (v_mfma_i32_16x16x64_i8 or v_mfma_f32_16x16x32_f16).  A stage is 128 bytes of an int8 reduction, 64 steps of a
-// 16-bit one, in two buffers, filled by buffer_load ... lds while the other one is multiplied.  An operand lies in a stage
+// 16-bit one, in a ring of buffers, filled by buffer_load ... lds while others are multiplied.  An operand lies in a stage
 //   kFast    as whole 128-byte lines of its rows, 16-byte pieces XOR-swizzled by row / 2 so that the 16 rows a fragment read takes lie
 //            in different banks
 //   kSlow16  as stored with a slow reduction index, 64 steps of 16-bit columns, transposed by ds_read_b64_tr_b16, its 32-byte pieces
 //            XOR-swizzled by the step
 //   kSlow8   the same of int8 columns, transposed by ds_read_b64_tr_b8 and made 16-bit floats in registers (exact)
 //
-// What bounds the large tile (8192 x 8192 x 4096, 512 tiles, 2.1 GHz): a stage's products alone take 2048 clocks, its loads pass at 64
-// bytes a clock (64 KB: 1024), its fragments are 192 KB of LDS reads.  Gradient sums 393 - 423 us; with the loads left out 360 - 380, with
-// products alone 307 - 335; loads issued all at once behind the barrier 425 - 464.
+// What bounds the 256 x 256 tile is the matrix units' power more than its schedule: over 8192 x 8192 x 4096 the statistics, a piece of
+// the gradient and the two sums took 264, 235, 430 and 390 us on data and 189, 180, 312 and 297 us, in the same code, on zeros.  What was
+// measured on the way there, as sums of one gradient and of the other: loads issued all at once behind the barrier 464 and 437, spread
+// over the products of half a stage 427 and 393; with the loads left out 381 and 359, with products alone 335 and 308; two phases of half
+// the rows with a barrier each 446 and 407; four wavefronts of 128 x 128, whose sums move between register files, 635 and 589.
 #include "lds_asm.h"
 #include "vocab.h"
 
@@ -476,6 +478,7 @@ __device__ inline v4i row_piece(const char* p, int left) {
 constexpr int kPlaces = 8;     // of a row, whose products a wavefront makes at a time
 
 // Logits of the targets: a wavefront takes eight places of a row, its lanes sixteen features each, the loads of all in flight together.
+// Bound by the gathered rows' way: 64 places of 8192 rows of 2048 features 139 us, 1.07 GB at 7.7 TB/s, most of it out of the caches.
 __device__ inline void dots_block(const VocabLogits& l, const VocabTargets& t, int block, int waves) {
   const int lane = threadIdx.x & 63;
   const int groups = (t.top + kPlaces - 1) / kPlaces;
@@ -567,6 +570,9 @@ __device__ inline void stats_of(const VocabLogits& l, const VocabStats& st, cons
   }
 }
 
+// Bound by the products: 8192 rows of 4096 features over 131072 classes 3.37 ms, 2.6 POP/s; few rows by the weights' way: 16 rows over
+// 32000 classes of 4096 21 us, 131 MB at 6.2 TB/s called again and again, partly out of the last-level cache.  A pair per row and tile of
+// classes is all that leaves.
 // Statistics of the tiles, or - the first `others` workgroups, a multiple of eight - the targets' logits, which depend on nothing else
 // either.  Large tiles: each workgroup takes several in turn.
 template <class T>
@@ -661,6 +667,8 @@ __device__ inline uint64_t grad_of(v4i s, v4i row, float k, int v, int classes) 
 }
 __device__ inline uint16_t target_grad(int bits) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(ldexpf(__int_as_float(bits), kGradExponent))); }
 
+// A piece of the gradient.  Bound as the statistics: 8192 rows of 4096 features, 8192 classes 249 us (2.2 POP/s), 134 MB out among it;
+// few rows by one workgroup's walk from its start to the last store.
 template <class T>
 __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(const VocabLogits l, const VocabGrad g) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -849,6 +857,9 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
   }
 }
 
+// Bound by the products where rows are many: 8192 x 4096, 8192 classes 809 us for both (1.36 PFLOP/s; the library's product reaches
+// 1.43), by memory where they are few: 31 x 4096 over 32000 70 us, 393 MB at 5.6 TB/s.  Sums of 32 bits; what is 16 bits wide on the way
+// in has eleven significant ones.
 // Both gradients' sums: the first `blocks_a` workgroups (a multiple of eight, see tile_of) the activations', the others the weights'.  The
 // large tile reads a 16-bit copy of the int8 weights: made 16-bit in registers its fragments take 487 us of 8192 x 8192 x 4096, read from
 // the copy 435, and the copy is 20 us of workgroups in the shadow of another launch.
@@ -860,7 +871,7 @@ __global__ __launch_bounds__(TA::kThreads, TW::kPerUnit) void vocab_sums_kernel(
   else sums_tile<TW, kSlow16, kSlow16>(w, blockIdx.x - blocks_a, smem);
 }
 
-// adds the slices, scales, rounds; a lane takes four neighbours of a row
+// Adds the slices, scales, rounds; a lane takes four neighbours of a row.  Bound by memory: 8192 x 4096 in one part 44 us, 201 MB at 4.6 TB/s
 __device__ inline void join_block(const VocabSums& s, long long block) {
   const int quads = (s.ni + 3) / 4;
   const long long at = block * 256 + threadIdx.x, all = static_cast<long long>(quads) * s.nj;
