@@ -28,12 +28,14 @@ constexpr int kNone = -2147483647 - 1;                // below every logit
 enum Layout { kFast, kSlow16, kSlow8 };
 constexpr int stage_bytes(int r, Layout l) { return l == kSlow8 ? 64 * r : kStageBytes * r; }
 
-template <int TI_, int TJ_, int WI_, int WJ_, int RING_, int PER_UNIT>
+template <int TI_, int TJ_, int WI_, int WJ_, int RING_, int PER_UNIT, bool APART = false>
 struct Tile {
   static constexpr int TI = TI_, TJ = TJ_, WI = WI_, WJ = WJ_, RING = RING_;     // RING: buffers
   static constexpr int kWaves = WI * WJ, kThreads = 64 * kWaves;
   static constexpr int BI = TI / WI / 16, BJ = TJ / WJ / 16;   // 16 x 16 blocks of a wavefront
-  static constexpr int kLds = RING * (TI + TJ) * kStageBytes;
+  static constexpr bool kApart = APART;                        // see Apart
+  static constexpr int kRings = kApart ? kWaves : 1;
+  static constexpr int kLds = kRings * RING * (TI + TJ) * kStageBytes;
   static constexpr int kPerUnit = PER_UNIT;      // workgroups per unit that the registers are cut for
   static constexpr bool kInTurn = TI == 256;     // logits: a workgroup takes several tiles in turn, with LDS for their ends behind the ring
   static constexpr int kLdsLogits = kLds + (kInTurn ? 2 * TI * 16 * WJ : 0);
@@ -44,6 +46,8 @@ typedef Tile<64, 64, 2, 2, 2, 4> TileSmall;
 typedef Tile<64, 64, 2, 2, 4, 2> TileDeep;      // few tiles: what counts is how soon the loads are out
 typedef Tile<128, 32, 4, 1, 4, 2> TileFew;
 typedef Tile<128, 32, 4, 1, 3, 4> TileFewSums;
+typedef Tile<64, 32, 4, 1, 3, 2, true> TileFewApart;      // few tiles of long reductions: a stage of the reduction for each wavefront
+typedef Tile<64, 64, 2, 2, 2, 2, true> TileSmallApart;
 typedef Tile<128, 128, 2, 2, 1, 4> TileShort;   // short reductions: nothing overlaps within a tile, but with three other tiles of a unit
 
 // 16-lane groups: lane i of a group names 8 bytes of a 4 x 16 block of 16-bit values (row i / 4, columns 4 (i % 4) .. + 4) and receives
@@ -100,14 +104,14 @@ struct Source {
 
   __device__ void lanes(const VocabOperand& o) {
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     piece = 0;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
       const int row = (q * kWaves + wave) * kRowsPerLoad + lane / kPieces;
       const int slot = lane % kPieces;
       const int c = L == kFast ? slot ^ ((row >> 1) & 7) : (L == kSlow16 ? slot ^ (2 * turn(row)) : slot ^ turn(row));
-      if (!kSlow) piece = c * 16;       // the same for every q: a load's rows are a multiple of 16 apart
+      if (!kSlow && q == 0) piece = c * 16;
       voff[q] = static_cast<int>(row * o.pitch) + c * 16;
     }
   }
@@ -135,13 +139,15 @@ struct Source {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, n, 0x00020000);
   }
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned lds, int q) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, NITI_LDS_AT(lds + (q * kWaves + wave) * 1024), 16, kSlow || piece < fast_left ? voff[q] : kFar, 0, 0, 0);
+    const int wave = kWaves == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int turned = (q * kWaves * kRowsPerLoad / 2 & 7) << 4;      // rows of this load have their pieces turned by this against load 0's
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, NITI_LDS_AT(lds + (q * kWaves + wave) * 1024), 16, kSlow || (piece ^ turned) < fast_left ? voff[q] : kFar, 0, 0, 0);
   }
+  template <int BY = 1>
   __device__ void next() {
-    base += advance;
-    left -= advance;
-    fast_left -= kStageBytes;
+    base += BY * advance;
+    left -= BY * advance;
+    fast_left -= BY * kStageBytes;
   }
 };
 
@@ -380,6 +386,99 @@ struct Product {
   }
 };
 
+// The same sums where a launch is few tiles: what counts is a tile's walk along its reduction, stage after stage.  Each wavefront takes every
+// kWaves-th stage, for the whole tile, in a ring of its own and without barriers; their sums meet in LDS at the end, in the order of the
+// wavefronts, and go back to the registers as Product leaves them.
+template <class T, Layout LX, Layout LY, class Acc>
+struct Apart {
+  static constexpr int PI = T::TI / 16, PJ = T::TJ / 16;
+  Source<T::TI, LX, 1> sx;
+  Source<T::TJ, LY, 1> sy;
+  Fragments<T::TI, PI, LX> fx;
+  Fragments<T::TJ, PJ, LY> fy;
+  Acc acc[T::BI][T::BJ];
+  static constexpr int kStageX = stage_bytes(T::TI, LX), kStageY = stage_bytes(T::TJ, LY);
+  static constexpr int kStageLoads = Source<T::TI, LX, 1>::kLoads + Source<T::TJ, LY, 1>::kLoads;
+  static_assert(T::RING == 2 || T::RING == 3, "the waits");
+  static_assert(T::kWaves * PI * PJ * 1024 <= T::kWaves * T::RING * (kStageX + kStageY), "the sums meet where the rings were");
+
+  __device__ void issue(unsigned ldsx, unsigned ldsy, int buf) {
+    const __amdgpu_buffer_rsrc_t rx = sx.stage(), ry = sy.stage();
+    static_for<Source<T::TI, LX, 1>::kLoads>([&](auto q) { sx.load(rx, ldsx + buf * kStageX, decltype(q)::value); });
+    static_for<Source<T::TJ, LY, 1>::kLoads>([&](auto q) { sy.load(ry, ldsy + buf * kStageY, decltype(q)::value); });
+    sx.template next<T::kWaves>();
+    sy.template next<T::kWaves>();
+  }
+  __device__ void run(const VocabOperand& x, const VocabOperand& y, int i0, int j0, int k0, int n, int x_end, int y_end, char* smem) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const unsigned ldsx = lds_addr(smem) + wave * T::RING * (kStageX + kStageY), ldsy = ldsx + T::RING * kStageX;
+    sx.lanes(x);
+    sy.lanes(y);
+    fx.init(ldsx, 0);
+    fy.init(ldsy, 0);
+    sx.seek(x, i0, k0 + wave, x_end);
+    sy.seek(y, j0, k0 + wave, y_end);
+    Acc own[PI][PJ];
+#pragma unroll
+    for (int i = 0; i < PI; ++i)
+#pragma unroll
+      for (int j = 0; j < PJ; ++j) own[i][j] = Acc{0, 0, 0, 0};
+    const int rounds = (n - wave + T::kWaves - 1) / T::kWaves;      // stages of this wavefront
+    static_for<T::RING>([&](auto b) {
+      if (decltype(b)::value < rounds) issue(ldsx, ldsy, decltype(b)::value);
+    });
+    int buf = 0;
+    for (int left = rounds - 1; left >= 0; --left) {      // stages behind this one, of which RING - 1 are under way
+      if (left >= T::RING - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::RING - 1) * kStageLoads) : "memory");
+      else if (left == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStageLoads) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      static_for<2>([&](auto h) {
+        constexpr int H = decltype(h)::value;
+        static_for<PJ>([&](auto j) { fy.template read<H, decltype(j)::value>(); });
+        static_for<PI>([&](auto i) { fx.template read<H, decltype(i)::value>(); });
+      });
+      lds_settle<0>();
+      fx.template landed<0>();
+      fx.template landed<1>();
+      fy.template landed<0>();
+      fy.template landed<1>();
+      if (left >= T::RING) issue(ldsx, ldsy, buf);
+      static_for<2>([&](auto h) {
+        constexpr int H = decltype(h)::value;
+        static_for<PI>([&](auto i) {
+          constexpr int I = decltype(i)::value;
+          const v4i xi = fx.template get<H, I>();
+          static_for<PJ>([&](auto j) { own[I][decltype(j)::value] = multiply(xi, fy.template get<H, decltype(j)::value>(), own[I][decltype(j)::value]); });
+        });
+      });
+      const int step = buf + 1 < T::RING ? 1 : 1 - T::RING;
+      fx.other_buffer(step * kStageX);
+      fy.other_buffer(step * kStageY);
+      buf += step;
+    }
+    tile_sync();
+    Acc* const meet = reinterpret_cast<Acc*>(smem) + lane;
+#pragma unroll
+    for (int i = 0; i < PI; ++i)
+#pragma unroll
+      for (int j = 0; j < PJ; ++j) meet[((wave * PI + i) * PJ + j) * 64] = own[i][j];
+    __syncthreads();
+    const int wi = wave / T::WJ, wj = wave % T::WJ;
+#pragma unroll
+    for (int i = 0; i < T::BI; ++i)
+#pragma unroll
+      for (int j = 0; j < T::BJ; ++j) {
+        const int at = (wi * T::BI + i) * PJ + wj * T::BJ + j;
+        acc[i][j] = meet[at * 64];
+#pragma unroll
+        for (int w = 1; w < T::kWaves; ++w) acc[i][j] += meet[(w * PI * PJ + at) * 64];
+      }
+    __syncthreads();
+  }
+};
+template <class T, Layout LX, Layout LY, class Acc>
+using Sums = std::conditional_t<T::kApart, Apart<T, LX, LY, Acc>, Product<T, LX, LY, Acc>>;
+
 // Workgroup -> tile: a die (every eighth workgroup) takes a run of tiles, and a run goes down `kRows` tile rows before the next column,
 // so that the tiles in flight on a die share their operands in its L2.
 __device__ inline void tile_of(int block, int ti, int tj, int* i, int* j) {
@@ -594,7 +693,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_stats_kernel(c
   } else {
     int bi, bj;
     tile_of(block, ti, tj, &bi, &bj);
-    Product<T, kFast, kFast, v4i> p;
+    Sums<T, kFast, kFast, v4i> p;
     p.run(l.w, l.a, bi * T::TI, bj * T::TJ, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
     stats_of<T>(l, st, p.acc, k, bi * T::TI, bj * T::TJ, bi, reinterpret_cast<int2*>(smem));
   }
@@ -741,7 +840,7 @@ __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(co
     int2 place = make_int2(0, -1);
     int place_row = 0;
     if (kEarly && static_cast<int>(threadIdx.x) < places) place = place_of(threadIdx.x, &place_row);
-    Product<T, kFast, kFast, v4i> p;
+    Sums<T, kFast, kFast, v4i> p;
     p.run(l.w, l.a, i0, j0, 0, (l.features + kStageBytes - 1) / kStageBytes, l.w.row_bytes, l.a.row_bytes, smem);
     const Outgoing<T> out{smem};
     if constexpr (!kEarly) {
@@ -790,7 +889,7 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
   const int n = min(s.steps, stages - k0);
   const int end = min(s.nk, (k0 + n) * 64);      // steps
   const int e = sums_exponent(s);
-  Product<T, LX, LY, v4f> p;
+  Sums<T, LX, LY, v4f> p;
   p.run(s.x, s.y, i0, j0, k0, n, LX == kFast ? 2 * ((end + 7) & ~7) : end, LY == kFast ? 2 * ((end + 7) & ~7) : end, smem);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -864,7 +963,7 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
 // large tile reads a 16-bit copy of the int8 weights: made 16-bit in registers its fragments take 487 us of 8192 x 8192 x 4096, read from
 // the copy 435, and the copy is 20 us of workgroups in the shadow of another launch.
 template <class TA, class TW>
-__global__ __launch_bounds__(TA::kThreads, TW::kPerUnit) void vocab_sums_kernel(const VocabSums a, const VocabSums w, int blocks_a) {
+__global__ __launch_bounds__(TA::kThreads, TA::kPerUnit < TW::kPerUnit ? TA::kPerUnit : TW::kPerUnit) void vocab_sums_kernel(const VocabSums a, const VocabSums w, int blocks_a) {
   static_assert(TA::kThreads == TW::kThreads, "one launch");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   if (static_cast<int>(blockIdx.x) < blocks_a) sums_tile<TA, TA::TI == 256 ? kSlow16 : kSlow8, kFast>(a, blockIdx.x, smem);
@@ -954,7 +1053,7 @@ int run_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
 }
 template <class TA, class TW>
 int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
-  constexpr int kLdsA = TA::RING * (stage_bytes(TA::TI, TA::TI == 256 ? kSlow16 : kSlow8) + stage_bytes(TA::TJ, kFast)), kOutA = 2 * TA::TI * TA::TJ;
+  constexpr int kLdsA = TA::kRings * TA::RING * (stage_bytes(TA::TI, TA::TI == 256 ? kSlow16 : kSlow8) + stage_bytes(TA::TJ, kFast)), kOutA = 2 * TA::TI * TA::TJ;
   constexpr int kMostA = kLdsA > kOutA ? kLdsA : kOutA, kLds = kMostA > TW::kLds ? kMostA : TW::kLds;
   if (const int rc = with_lds<vocab_sums_kernel<TA, TW>>(kLds, "vocab_sums")) return rc;
   const long long na = (tiles_of(a.ni, a.nj, TA::TI, TA::TJ) * a.slices + 7) / 8 * 8, nw = tiles_of(w.ni, w.nj, TW::TI, TW::TJ) * w.slices;
@@ -966,13 +1065,18 @@ int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
 }  // namespace
 
 // By statistics and gradients of 60 sizes (64 to 8192 rows, 512 to 100096 classes, 64 to 2048 features) with each tile.
+//   Up to 32 rows, 64 x 32 and a stage for each wavefront where every tile has a unit and there is more than one stage for each:
+//   30 x 2304 over 720 5.7 us (128 x 32 8.3), 1 x 4096 over 1000 7.2 (12.1), 16 x 1024 over 10000 5.1 (5.7), 2 x 128 over 64 4.0 (3.5)
+//   64 x 64 and a stage for each wavefront likewise: 100 x 4096 over 504 8.7 (64 x 64 together 11.0), 64 x 2048 over 4000 6.6 (7.2), 400 x 2560 over
+//   2800, 308 tiles, 12.8 (10.1)
 //   64 x 64 where the device holds them all at once: 64 rows of 64 features over 20032 classes 4.4 us (128 x 128 4.9), of 2048 11 (16)
 //   128 x 128 in a ring of two, two to a unit, where the device holds these at once and there are stages to overlap: 256 x 1024 over 10048 8.7
 //   (one buffer and four to a unit 11.2), 256 x 256 5.6 (5.9), 256 x 64 5.0 (4.9)
 //   256 x 256 in turn for long reductions on many rounds: a round is 1.68 of 128 x 128.  2048 x 2048 over 32064 141 (157), x 1024 79 (78), x 512 52 (48)
 //   128 x 128 in one buffer, four to a unit, elsewhere: 1024 x 64 over 100096 41 (256 x 256 55, ring of two 60), 300 x 1024 over 30016 17 (22, 20)
 VocabTile vocab_logits_tile(int rows, int features, int classes) {
-  if (rows <= 32) return kVocabFew;
+  if (rows <= 32) return features >= 512 && tiles_of(classes, rows, 64, 32) <= 256 ? kVocabFewApart : kVocabFew;
+  if (features > 1024 && tiles_of(classes, rows, 64, 64) <= 256) return kVocabSmallApart;
   if (tiles_of(classes, rows, 64, 64) <= 512) return kVocabSmall;
   const double middle = static_cast<double>(tiles_of(classes, rows, 128, 128)) / 512;
   if (middle <= 1.0) return features >= 512 ? kVocabMiddle : kVocabQuad;
@@ -981,8 +1085,9 @@ VocabTile vocab_logits_tile(int rows, int features, int classes) {
 }
 
 int vocab_stats_tiles(VocabTile t, int classes) {
-  const int classes_of_tile = t == kVocabLarge ? TileLarge::TI : (t == kVocabSmall ? TileDeep::TI : TileMiddle::TI);
-  static_assert(TileMiddle::TI == TileFew::TI, "one rule");
+  const bool narrow = t == kVocabSmall || t == kVocabSmallApart || t == kVocabFewApart;
+  const int classes_of_tile = t == kVocabLarge ? TileLarge::TI : (narrow ? TileDeep::TI : TileMiddle::TI);
+  static_assert(TileMiddle::TI == TileFew::TI && TileDeep::TI == TileFewApart::TI && TileDeep::TI == TileSmallApart::TI, "one rule");
   return (classes + classes_of_tile - 1) / classes_of_tile;
 }
 
@@ -992,6 +1097,8 @@ int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, c
     case kVocabMiddle: return run_stats<TileMiddle>(l, s, targets, stream);
     case kVocabSmall: return run_stats<TileDeep>(l, s, targets, stream);
     case kVocabQuad: return run_stats<TileShort>(l, s, targets, stream);
+    case kVocabSmallApart: return run_stats<TileSmallApart>(l, s, targets, stream);
+    case kVocabFewApart: return run_stats<TileFewApart>(l, s, targets, stream);
     default: return run_stats<TileFew>(l, s, targets, stream);
   }
 }
@@ -999,7 +1106,7 @@ int launch_vocab_stats(VocabTile t, const VocabLogits& l, const VocabStats& s, c
 bool vocab_sums_wants_wide_weights(VocabTile t) { return t == kVocabLarge; }
 
 // a tile looks through the places of all of its rows: up to sixteen rounds of its threads.  Large ones have no registers for it
-bool vocab_grad_writes_targets(VocabTile t, int top) { return t != kVocabLarge && top <= (t == kVocabFew ? 128 : 32); }
+bool vocab_grad_writes_targets(VocabTile t, int top) { return t != kVocabLarge && top <= (t == kVocabFew || t == kVocabFewApart ? 128 : 32); }
 
 int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
   switch (t) {
@@ -1007,6 +1114,8 @@ int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hip
     case kVocabMiddle: return run_grad<TileMiddle>(l, g, stream);
     case kVocabSmall: return run_grad<TileDeep>(l, g, stream);
     case kVocabQuad: return run_grad<TileShort>(l, g, stream);
+    case kVocabSmallApart: return run_grad<TileSmallApart>(l, g, stream);
+    case kVocabFewApart: return run_grad<TileFewApart>(l, g, stream);
     default: return run_grad<TileFew>(l, g, stream);
   }
 }
@@ -1030,6 +1139,8 @@ constexpr SumsCosts kSumsCosts[] = {
     {kVocabQuad, 33, 0x7fffffff, {128, 128, 1024, 1.4, 6.0}, {128, 128, 1024, 1.2, 6.0}},
     {kVocabSmall, 33, 0x7fffffff, {64, 64, 1024, 0.7, 3.7}, {64, 64, 1024, 0.84, 3.0}},
     {kVocabShort, 33, 512, {64, 64, 1024, 0.61, 2.85}, {128, 128, 1024, 1.2, 6.8}},
+    {kVocabSmallApart, 33, 512, {64, 64, 256, 0.25, 4.2}, {128, 128, 256, 1.2, 3.4}},
+    {kVocabFewApart, 1, 32, {64, 32, 256, 0.11, 3.9}, {128, 128, 256, 1.0, 3.5}},
     {kVocabFew, 1, 32, {128, 32, 1024, 0.24, 3.0}, {128, 128, 1024, 1.0, 1.9}},
 };
 }  // namespace
@@ -1073,6 +1184,8 @@ int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipSt
     case kVocabSmall: return run_sums<TileSmall, TileSmall>(a, w, stream);
     case kVocabShort: return run_sums<TileSmall, TileShort>(a, w, stream);
     case kVocabQuad: return run_sums<TileShort, TileShort>(a, w, stream);
+    case kVocabSmallApart: return run_sums<TileSmallApart, TileShort>(a, w, stream);
+    case kVocabFewApart: return run_sums<TileFewApart, TileShort>(a, w, stream);
     default: return run_sums<TileFewSums, TileShort>(a, w, stream);
   }
 }

@@ -136,6 +136,15 @@ def test_long_reductions_are_cut(dev, n, f, v):
     run("entropy", dev, n, f, v, seed=n)
 
 
+# few tiles of long reductions: features and classes that end inside a stage, fewer stages than wavefronts and no multiple of them
+@pytest.mark.parametrize("n", [1, 17, 32, 33, 65])
+@pytest.mark.parametrize("f,v", [(512, 64), (528, 1000), (1041, 333), (1100, 4100), (1552, 65), (2304, 721), (4100, 1500)])
+def test_few_tiles_of_long_reductions(dev, n, f, v):
+    print("long", n, f, v, flush=True)
+    run("entropy", dev, n, f, v, seed=n + f)
+    run("distill", dev, n, f, v, t=2.0, k=5, seed=n + v, weight=torch.rand(n, device=dev))
+
+
 @pytest.mark.parametrize("n", [20, 300])
 def test_row_weights(dev, n):
     g = _gen(dev, n)
