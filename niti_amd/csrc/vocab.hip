@@ -386,9 +386,10 @@ struct Product {
   }
 };
 
-// The same sums where a launch is few tiles: what counts is a tile's walk along its reduction, stage after stage.  Each wavefront takes every
-// kWaves-th stage, for the whole tile, in a ring of its own and without barriers; their sums meet in LDS at the end, in the order of the
-// wavefronts, and go back to the registers as Product leaves them.
+// The same sums where a launch is few tiles: what counts is a tile's walk along its reduction, 0.3 - 0.4 us a stage where wavefronts take
+// stages together (barrier, fragments and products one after the other; a ring of eight is no faster).  Each takes every kWaves-th stage
+// here, for the whole tile, in a ring of its own and without barriers; their sums meet in LDS at the end, in the order of the wavefronts, and
+// go back to the registers as Product leaves them.  Sums of a tile of 16 x 512 over 1000 classes, 16 stages, 6.7 us together.
 template <class T, Layout LX, Layout LY, class Acc>
 struct Apart {
   static constexpr int PI = T::TI / 16, PJ = T::TJ / 16;
@@ -1067,8 +1068,8 @@ int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
 // By statistics and gradients of 60 sizes (64 to 8192 rows, 512 to 100096 classes, 64 to 2048 features) with each tile.
 //   Up to 32 rows, 64 x 32 and a stage for each wavefront where every tile has a unit and there is more than one stage for each:
 //   30 x 2304 over 720 5.7 us (128 x 32 8.3), 1 x 4096 over 1000 7.2 (12.1), 16 x 1024 over 10000 5.1 (5.7), 2 x 128 over 64 4.0 (3.5)
-//   64 x 64 and a stage for each wavefront likewise: 100 x 4096 over 504 8.7 (64 x 64 together 11.0), 64 x 2048 over 4000 6.6 (7.2), 400 x 2560 over
-//   2800, 308 tiles, 12.8 (10.1)
+//   64 x 64 and a stage for each wavefront likewise, the targets' workgroups beside the tiles counted: 100 x 4096 over 504 8.7 (64 x 64 together
+//   11.0), 500 x 2304 over 1000 7.1 (7.9), 256 x 1536 over 4000, 252 tiles and 64, 8.2 (6.8)
 //   64 x 64 where the device holds them all at once: 64 rows of 64 features over 20032 classes 4.4 us (128 x 128 4.9), of 2048 11 (16)
 //   128 x 128 in a ring of two, two to a unit, where the device holds these at once and there are stages to overlap: 256 x 1024 over 10048 8.7
 //   (one buffer and four to a unit 11.2), 256 x 256 5.6 (5.9), 256 x 64 5.0 (4.9)
@@ -1076,7 +1077,7 @@ int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
 //   128 x 128 in one buffer, four to a unit, elsewhere: 1024 x 64 over 100096 41 (256 x 256 55, ring of two 60), 300 x 1024 over 30016 17 (22, 20)
 VocabTile vocab_logits_tile(int rows, int features, int classes) {
   if (rows <= 32) return features >= 512 && tiles_of(classes, rows, 64, 32) <= 256 ? kVocabFewApart : kVocabFew;
-  if (features > 1024 && tiles_of(classes, rows, 64, 64) <= 256) return kVocabSmallApart;
+  if (features > 1024 && tiles_of(classes, rows, 64, 64) + (rows + 3) / 4 <= 256) return kVocabSmallApart;
   if (tiles_of(classes, rows, 64, 64) <= 512) return kVocabSmall;
   const double middle = static_cast<double>(tiles_of(classes, rows, 128, 128)) / 512;
   if (middle <= 1.0) return features >= 512 ? kVocabMiddle : kVocabQuad;
