@@ -670,7 +670,7 @@ __device__ inline void stats_of(const VocabLogits& l, const VocabStats& st, cons
   }
 }
 
-// Bound by the products: 8192 rows of 4096 features over 131072 classes 3.37 ms, 2.6 POP/s; few rows by the weights' way: 16 rows over
+// Bound by the products: 8192 rows of 4096 features over 131072 classes 3.14 - 3.37 ms on two cards, 2.6 - 2.8 POP/s; few rows by the weights' way: 16 rows over
 // 32000 classes of 4096 21 us, 131 MB at 6.2 TB/s called again and again, partly out of the last-level cache.  A pair per row and tile of
 // classes is all that leaves.
 // Statistics of the tiles, or - the first `others` workgroups, a multiple of eight - the targets' logits, which depend on nothing else
@@ -767,7 +767,7 @@ __device__ inline uint64_t grad_of(v4i s, v4i row, float k, int v, int classes) 
 }
 __device__ inline uint16_t target_grad(int bits) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(ldexpf(__int_as_float(bits), kGradExponent))); }
 
-// A piece of the gradient.  Bound as the statistics: 8192 rows of 4096 features, 8192 classes 249 us (2.2 POP/s), 134 MB out among it;
+// A piece of the gradient.  Bound as the statistics: 8192 rows of 4096 features, 8192 classes 241 - 249 us (2.2 - 2.3 POP/s), 134 MB out among it;
 // few rows by one workgroup's walk from its start to the last store.
 template <class T>
 __global__ __launch_bounds__(T::kThreads, T::kPerUnit) void vocab_grad_kernel(const VocabLogits l, const VocabGrad g) {
@@ -957,7 +957,7 @@ __device__ inline void sums_tile(const VocabSums& s, int block, char* smem) {
   }
 }
 
-// Bound by the products where rows are many: 8192 x 4096, 8192 classes 809 us for both (1.36 PFLOP/s; the library's product reaches
+// Bound by the products where rows are many: 8192 x 4096, 8192 classes 766 - 809 us for both (1.36 - 1.43 PFLOP/s; the library's product reaches
 // 1.43), by memory where they are few: 31 x 4096 over 32000 70 us, 393 MB at 5.6 TB/s.  Sums of 32 bits; what is 16 bits wide on the way
 // in has eleven significant ones.
 // Both gradients' sums: the first `blocks_a` workgroups (a multiple of eight, see tile_of) the activations', the others the weights'.  The
@@ -1124,7 +1124,8 @@ int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hip
 namespace {
 // What a workgroup of the sums takes, in us: per stage and beside them, with as many of its kind on the device as `slots`.  Fitted, with
 // the two terms of the parts' adding below, to the times of every tile and cut for 35 sizes (1 to 8192 rows, 64 to 4096 features, 100 to 60032
-// classes, some 1400 combinations): what the plan picks is at most 4 % off the best of them.
+// classes, some 1400 combinations): what the plan picks is at most 4 % off the best of them.  The wavefronts' own stages (the two ...Apart)
+// were fitted later, to 26 sizes of 1 to 400 rows: 16 x 512 over 2000 7.6 us (128 x 32 13.6), 128 x 512 over 1000 7.0 (8.7).
 struct SumsCost {
   int ti, tj, slots;
   double stage, fixed;
