@@ -370,7 +370,7 @@ def vocab_backward(act, w, exp_a, exp_w, state, grad=None):
     act 2^exp_a and w 2^exp_w: (d_act like act, d_w [V,F]) as bfloat16, summed in float32.  ``grad``: float32, one value or one per
     row; None: 1.  The softmax is computed again, a piece of the classes at a time, and held as float16 (scaled: eleven bits down
     to 2^-29), so the gradients carry three roundings more than the sums: that of p - q to eleven bits, d_w's of grad act to
-    eleven, and the result's to eight."""
+    eleven (fewer where a row's grad is below 2^-22 of the largest), and the result's to eight."""
     return L.host().vocab_backward(act, w, exp_a, exp_w, state.rows, state.top, state.temperature, grad)
 
 
