@@ -597,7 +597,8 @@ int niti_group_conv_i8_f32(const int8_t* x, const int8_t* w, float* y, int N, in
  *
  * Both leave in `state` (rows * niti_vocab_state_words(top) int32, 16-byte aligned; top = 1 for the entropy) what niti_vocab_backward_i8 needs: gradients
  * of sum_n weight[n] loss[n] with respect to act 2^exp_a (d_act [rows][features]) and w 2^exp_w (d_w [classes][features]) as bfloat16, from
- * sums in float32.  weight: `weights` = rows values, one for all, or null for 1.  The logits are computed again, a piece of the
+ * sums in float32; niti_vocab_backward_i8_f32 leaves these sums as float32 (for what rounds them itself: a rounding that takes a gradient's low bits for random
+ * numbers finds none in bfloat16).  weight: `weights` = rows values, one for all, or null for 1.  The logits are computed again, a piece of the
  * classes at a time; the softmax of a piece, times 2^15, and weight[n] act, over a power of two, are held as float16.
  *
  * The workspaces depend on the operands' addresses through their alignment alone.
@@ -606,6 +607,7 @@ enum { NITI_F32 = 0, NITI_BF16 = 1, NITI_F16 = 2 };
 size_t niti_vocab_state_words(int top);
 size_t niti_vocab_forward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes);
 size_t niti_vocab_backward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes);
+size_t niti_vocab_backward_f32_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes);
 int niti_vocab_entropy_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w,
                           int rows, int features, int classes, const void* target, int target_bytes, int64_t ignored, float* loss, float* lse,
                           int32_t* state, void* workspace, size_t workspace_bytes, void* stream);
@@ -616,6 +618,9 @@ int niti_vocab_distill_i8(const int8_t* act, int64_t act_pitch, const int8_t* w,
 int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w,
                            int rows, int features, int classes, int top, float temperature, const int32_t* state, const float* weight,
                            int weights, uint16_t* d_act, uint16_t* d_w, void* workspace, size_t workspace_bytes, void* stream);
+int niti_vocab_backward_i8_f32(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                               int features, int classes, int top, float temperature, const int32_t* state, const float* weight,
+                               int weights, float* d_act, float* d_w, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ==================================================================================================================
  * MEASUREMENT ONLY - not part of the boundary a reference checkout binds to; nothing in the layers calls it.

@@ -101,9 +101,11 @@ SIGNATURES = {
     "niti_vocab_state_words": (_sz, [_i]),
     "niti_vocab_forward_workspace": (_sz, [_vp, _i64, _vp, _i64] + [_i] * 3),
     "niti_vocab_backward_workspace": (_sz, [_vp, _i64, _vp, _i64] + [_i] * 3),
+    "niti_vocab_backward_f32_workspace": (_sz, [_vp, _i64, _vp, _i64] + [_i] * 3),
     "niti_vocab_entropy_i8": (_i, [_vp, _i64, _vp, _i64, _vp, _vp] + [_i] * 3 + [_vp, _i, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "niti_vocab_distill_i8": (_i, [_vp, _i64, _vp, _i64, _vp, _vp] + [_i] * 3 + [_vp, _i, _vp, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _sz, _vp]),
     "niti_vocab_backward_i8": (_i, [_vp, _i64, _vp, _i64, _vp, _vp] + [_i] * 4 + [C.c_float, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
+    "niti_vocab_backward_i8_f32": (_i, [_vp, _i64, _vp, _i64, _vp, _vp] + [_i] * 4 + [C.c_float, _vp, _vp, _i, _vp, _vp, _vp, _sz, _vp]),
     "niti_mfma_probe_i8": (_i, [_vp, _sz, _i, _i, _vp, _vp, _vp]),
     "niti_mfma_probe_i8_16x16x64": (_i, [_vp, _sz, _i, _i, _vp, _vp, _vp]),
     "niti_group_conv_i8_f32": (_i, [_vp, _vp, _vp] + [_i] * 12 + [_vp]),

@@ -101,10 +101,10 @@ PyObject* forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// vocab_backward(act, w, exp_a, exp_w, state, places, temperature, weight or None) -> (d_act, d_w)
+// vocab_backward(act, w, exp_a, exp_w, state, places, temperature, weight or None, float32) -> (d_act, d_w)
 PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args g(args, n, 8, "vocab_backward");
+    Args g(args, n, 9, "vocab_backward");
     const at::Tensor& act = g.strided();
     const at::Tensor& w = g.strided();
     Opt ea = g.exponent(), ew = g.exponent();
@@ -112,6 +112,7 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int top = g.i();
     const double t = g.number();
     Opt weight = g.opt();
+    const bool f32 = g.flag();
     const char* const who = "vocab_backward";
     const Call c = call_of(act, w, ea, ew, who);
     same_device(act, {&w, ea, ew, &state, weight}, who);
@@ -119,17 +120,24 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
       refuse("vocab_backward: the state that the forward call of these rows returned expected");
     if (weight != nullptr && (weight->scalar_type() != at::kFloat || (weight->numel() != 1 && weight->sizes() != act.sizes().slice(0, act.dim() - 1))))
       refuse("vocab_backward: grad must be one float32 value or one per row of act");
-    at::Tensor da = empty(act.sizes(), at::kBFloat16, act), dw = empty(w.sizes(), at::kBFloat16, act);
+    const at::ScalarType type = f32 ? at::kFloat : at::kBFloat16;
+    at::Tensor da = empty(act.sizes(), type, act), dw = empty(w.sizes(), type, act);
     if (c.rows == 0) {
       dw.zero_();
       return tuple_of({da, dw});
     }
-    const size_t need = niti_vocab_backward_workspace(c.a.p, c.a.pitch, c.w.p, c.w.pitch, c.rows, c.features, c.classes);
+    const auto workspace_of = f32 ? niti_vocab_backward_f32_workspace : niti_vocab_backward_workspace;
+    const size_t need = workspace_of(c.a.p, c.a.pitch, c.w.p, c.w.pitch, c.rows, c.features, c.classes);
     const at::Tensor ws = workspace(need, act);
-    check(niti_vocab_backward_i8(c.a.p, c.a.pitch, c.w.p, c.w.pitch, ptr<int32_t>(ea), ptr<int32_t>(ew), c.rows, c.features, c.classes, top, static_cast<float>(t),
-                                 ptr<int32_t>(state), ptr<float>(weight), weight == nullptr ? 0 : static_cast<int>(weight->numel()), ptr<uint16_t>(da),
-                                 ptr<uint16_t>(dw), ws.data_ptr(), need, stream_of(act)),
-          "niti_vocab_backward_i8");
+    const int weights = weight == nullptr ? 0 : static_cast<int>(weight->numel());
+    if (f32)
+      check(niti_vocab_backward_i8_f32(c.a.p, c.a.pitch, c.w.p, c.w.pitch, ptr<int32_t>(ea), ptr<int32_t>(ew), c.rows, c.features, c.classes, top, static_cast<float>(t),
+                                       ptr<int32_t>(state), ptr<float>(weight), weights, ptr<float>(da), ptr<float>(dw), ws.data_ptr(), need, stream_of(act)),
+            "niti_vocab_backward_i8_f32");
+    else
+      check(niti_vocab_backward_i8(c.a.p, c.a.pitch, c.w.p, c.w.pitch, ptr<int32_t>(ea), ptr<int32_t>(ew), c.rows, c.features, c.classes, top, static_cast<float>(t),
+                                   ptr<int32_t>(state), ptr<float>(weight), weights, ptr<uint16_t>(da), ptr<uint16_t>(dw), ws.data_ptr(), need, stream_of(act)),
+            "niti_vocab_backward_i8");
     return tuple_of({da, dw});
   });
 }

@@ -126,6 +126,7 @@ struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
   long long part_pitch;
   int accumulate;            // add to what part holds
   uint16_t* out;             // bfloat16 [nj][ni]
+  float* out32;              // the same in float32 in its place, where it is not null (then part is not, either)
   // scale of the result: T 2^(exponent) weight
   float t;
   const int32_t* exponent;
@@ -149,6 +150,6 @@ int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hip
 // weights' (x: 16-bit activations, y: the piece's gradient, reduction slow in both)
 VocabTile vocab_sums_plan(int rows, int features, int classes, int* slices_a, int* steps_a, int* slices_w, int* steps_w);
 int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipStream_t stream);
-int launch_vocab_join(const VocabSums* a, const VocabSums* w, hipStream_t stream);   // either may be null
+int launch_vocab_join(const VocabSums* a, const VocabSums* w, hipStream_t stream);   // either may be null; those that write float32 go through here
 
 }  // namespace niti

@@ -241,7 +241,7 @@ struct BackwardPlan {
   int slices_a, steps_a, slices_w, steps_w;
   bool parts_a, parts_w;
 };
-BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
+BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features, bool f32) {
   BackwardPlan p{};
   Layout l;
   const long long row = round_up(features, 16);
@@ -257,8 +257,8 @@ BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features) {
   if (piece > round_up(w.rows, 8)) piece = round_up(w.rows, 8);
   p.piece = piece;
   p.tile = vocab_sums_plan(static_cast<int>(a.rows), features, static_cast<int>(piece), &p.slices_a, &p.steps_a, &p.slices_w, &p.steps_w);
-  p.parts_a = p.slices_a > 1 || piece < w.rows;
-  p.parts_w = p.slices_w > 1;
+  p.parts_a = f32 || p.slices_a > 1 || piece < w.rows;      // float32 results leave by way of the join
+  p.parts_w = f32 || p.slices_w > 1;
   p.a = l.take(p.copy_a ? a.rows * row : 0);
   p.w = l.take(p.copy_w ? w.rows * row : 0);
   p.wide_a = l.take(a.rows * p.pitch16 * 2);
@@ -321,55 +321,20 @@ int forward(const char* who, const int8_t* act, long long act_pitch, const int8_
   return check_launch(who);
 }
 
-}  // namespace
-}  // namespace niti
-
-using namespace niti;
-
-extern "C" size_t niti_vocab_state_words(int top) { return top > 0 ? static_cast<size_t>(vocab_state_words(top)) : 0; }
-
-extern "C" size_t niti_vocab_forward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
-  if (rows <= 0 || features <= 0 || classes <= 0) return 0;
-  return forward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features).bytes;
-}
-
-extern "C" size_t niti_vocab_backward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
-  if (rows <= 0 || features <= 0 || classes <= 0) return 0;
-  return backward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features).bytes;
-}
-
-extern "C" int niti_vocab_entropy_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
-                                     int features, int classes, const void* target, int target_bytes, int64_t ignored, float* loss, float* lse, int32_t* state,
-                                     void* workspace, size_t workspace_bytes, void* stream) {
-  clear_error();
-  return forward("vocab_entropy", act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, nullptr, 0, target, target_bytes, ignored, 1, 1.0f, loss, lse,
-                 state, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
-}
-
-extern "C" int niti_vocab_distill_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
-                                     int features, int classes, const void* top_value, int value_type, const void* top_class, int class_bytes, int top,
-                                     float temperature, float* loss, float* lse, int32_t* state, void* workspace, size_t workspace_bytes, void* stream) {
-  clear_error();
-  if (top_value == nullptr) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: null pointer");
-  if (value_type != NITI_F32 && value_type != NITI_BF16 && value_type != NITI_F16) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: value_type=%d", value_type);
-  if (!(temperature > 0.0f) || !isfinite(temperature)) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: temperature %g", static_cast<double>(temperature));
-  return forward("vocab_distill", act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top_value, value_type, top_class, class_bytes, -1, top, temperature,
-                 loss, lse, state, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
-}
-
-extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
-                                      int features, int classes, int top, float temperature, const int32_t* state, const float* weight, int weights,
-                                      uint16_t* d_act, uint16_t* d_w, void* workspace, size_t workspace_bytes, void* stream) {
-  clear_error();
+// d_act, d_w: bfloat16, or float32 by f32
+int backward(const int8_t* act, long long act_pitch, const int8_t* w, long long w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows, int features,
+             int classes, int top, float temperature, const int32_t* state, const float* weight, int weights, void* d_act, void* d_w, bool f32, void* workspace,
+             size_t workspace_bytes, hipStream_t st) {
   const char* const who = "vocab_backward";
-  hipStream_t const st = static_cast<hipStream_t>(stream);
+  const auto out16 = [f32](void* p, long long at) { return f32 ? nullptr : static_cast<uint16_t*>(p) + at; };
+  const auto out32 = [f32](void* p, long long at) { return f32 ? static_cast<float*>(p) + at : nullptr; };
   if (const int rc = check_operands(who, act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top)) return rc;
   if (state == nullptr || d_act == nullptr || d_w == nullptr) return fail(NITI_ERR_INVALID_ARG, "%s: null pointer", who);
   if (weight != nullptr && weights != 1 && weights != rows) return fail(NITI_ERR_INVALID_ARG, "%s: %d weights for %d rows", who, weights, rows);
   if (!(temperature > 0.0f) || !isfinite(temperature)) return fail(NITI_ERR_INVALID_ARG, "%s: temperature %g", who, static_cast<double>(temperature));
   if (!aligned16(state) || !aligned16(d_act) || !aligned16(d_w)) return fail(NITI_ERR_INVALID_ARG, "%s: state or result not 16-byte aligned", who);
   Matrix a{act, act_pitch, rows, features}, b{w, w_pitch, classes, features};
-  const BackwardPlan p = backward_plan(a, b, features);
+  const BackwardPlan p = backward_plan(a, b, features, f32);
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
     return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
   char* const ws = static_cast<char*>(workspace);
@@ -405,11 +370,11 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
     VocabSums sa{wide_weights ? VocabOperand{wide_w, p.pitch16 * 2, here, static_cast<int>(p.pitch16 * 2)}
                               : VocabOperand{piece.p, piece.pitch, here, piece.row_bytes},
                  VocabOperand{grad, p.piece * 2, rows, static_cast<int>(round_up(here, 8) * 2)}, features, rows, here, (stages + p.steps_a - 1) / p.steps_a, p.steps_a,
-                 p.parts_a ? reinterpret_cast<float*>(ws + p.part_a) : nullptr, p.part_pitch, first > 0 ? 1 : 0, d_act, temperature, exp_w, -kGradExponent, nullptr,
+                 p.parts_a ? reinterpret_cast<float*>(ws + p.part_a) : nullptr, p.part_pitch, first > 0 ? 1 : 0, out16(d_act, 0), out32(d_act, 0), temperature, exp_w, -kGradExponent, nullptr,
                  weight, weights};
     const VocabSums sw{VocabOperand{wide_a, p.pitch16 * 2, rows, static_cast<int>(p.pitch16 * 2)}, VocabOperand{grad, p.piece * 2, rows, static_cast<int>(p.piece * 2)},
                        features, here, rows, p.slices_w, p.steps_w, p.parts_w ? reinterpret_cast<float*>(ws + p.part_w) : nullptr, p.part_pitch, 0,
-                       d_w + first * features, temperature, exp_a, -kGradExponent - (each ? kRowExponent : 0), each ? exponent : nullptr, each ? nullptr : weight, 1};
+                       out16(d_w, first * features), out32(d_w, first * features), temperature, exp_a, -kGradExponent - (each ? kRowExponent : 0), each ? exponent : nullptr, each ? nullptr : weight, 1};
     if (const int rc = launch_vocab_sums(p.tile, sa, sw, st)) return rc;
     const bool join_a = p.parts_a && first + p.piece >= classes;
     sa.slices = p.slices_a;
@@ -418,4 +383,61 @@ extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, cons
     }
   }
   return NITI_OK;
+}
+
+}  // namespace
+}  // namespace niti
+
+using namespace niti;
+
+extern "C" size_t niti_vocab_state_words(int top) { return top > 0 ? static_cast<size_t>(vocab_state_words(top)) : 0; }
+
+extern "C" size_t niti_vocab_forward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
+  if (rows <= 0 || features <= 0 || classes <= 0) return 0;
+  return forward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features).bytes;
+}
+
+extern "C" size_t niti_vocab_backward_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
+  if (rows <= 0 || features <= 0 || classes <= 0) return 0;
+  return backward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features, false).bytes;
+}
+
+extern "C" size_t niti_vocab_backward_f32_workspace(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, int rows, int features, int classes) {
+  if (rows <= 0 || features <= 0 || classes <= 0) return 0;
+  return backward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features, true).bytes;
+}
+
+extern "C" int niti_vocab_entropy_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                                     int features, int classes, const void* target, int target_bytes, int64_t ignored, float* loss, float* lse, int32_t* state,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  return forward("vocab_entropy", act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, nullptr, 0, target, target_bytes, ignored, 1, 1.0f, loss, lse,
+                 state, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int niti_vocab_distill_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                                     int features, int classes, const void* top_value, int value_type, const void* top_class, int class_bytes, int top,
+                                     float temperature, float* loss, float* lse, int32_t* state, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (top_value == nullptr) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: null pointer");
+  if (value_type != NITI_F32 && value_type != NITI_BF16 && value_type != NITI_F16) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: value_type=%d", value_type);
+  if (!(temperature > 0.0f) || !isfinite(temperature)) return fail(NITI_ERR_INVALID_ARG, "vocab_distill: temperature %g", static_cast<double>(temperature));
+  return forward("vocab_distill", act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top_value, value_type, top_class, class_bytes, -1, top, temperature,
+                 loss, lse, state, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int niti_vocab_backward_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                                      int features, int classes, int top, float temperature, const int32_t* state, const float* weight, int weights,
+                                      uint16_t* d_act, uint16_t* d_w, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  return backward(act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top, temperature, state, weight, weights, d_act, d_w, false, workspace,
+                  workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int niti_vocab_backward_i8_f32(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
+                                          int features, int classes, int top, float temperature, const int32_t* state, const float* weight, int weights,
+                                          float* d_act, float* d_w, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  return backward(act, act_pitch, w, w_pitch, exp_a, exp_w, rows, features, classes, top, temperature, state, weight, weights, d_act, d_w, true, workspace,
+                  workspace_bytes, static_cast<hipStream_t>(stream));
 }

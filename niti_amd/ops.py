@@ -365,13 +365,16 @@ def vocab_distill(act, w, exp_a, exp_w, top_val, top_idx, temperature=1.0):
     return loss, lse, VocabState(rows, top_idx.shape[-1], temperature)
 
 
-def vocab_backward(act, w, exp_a, exp_w, state, grad=None):
+def vocab_backward(act, w, exp_a, exp_w, state, grad=None, dtype=torch.bfloat16):
     """Gradients of sum(grad * loss) of the vocab_loss or vocab_distill call that returned ``state``, with respect to the real values
-    act 2^exp_a and w 2^exp_w: (d_act like act, d_w [V,F]) as bfloat16, summed in float32.  ``grad``: float32, one value or one per
+    act 2^exp_a and w 2^exp_w: (d_act like act, d_w [V,F]) as ``dtype``, bfloat16 or float32, summed in float32.  ``grad``: float32, one value or one per
     row; None: 1.  The softmax is computed again, a piece of the classes at a time, and held as float16 (scaled: eleven bits down
     to 2^-29), so the gradients carry three roundings more than the sums: that of p - q to eleven bits, d_w's of grad act to
-    eleven (fewer where a row's grad is below 2^-22 of the largest), and the result's to eight."""
-    return L.host().vocab_backward(act, w, exp_a, exp_w, state.rows, state.top, state.temperature, grad)
+    eleven (fewer where a row's grad is below 2^-22 of the largest), and a bfloat16 result's to eight.  What rounds the result itself, and
+    by its low bits (PstoShift), wants float32."""
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError("vocab_backward: gradients as bfloat16 or float32")
+    return L.host().vocab_backward(act, w, exp_a, exp_w, state.rows, state.top, state.temperature, grad, dtype == torch.float32)
 
 
 def mask_features(x, mask, exp_in=None, exp_add=None):

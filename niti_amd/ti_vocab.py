@@ -19,12 +19,13 @@ def _power(n):
 
 def _fixed_point(x):
     """(int32 tensor, exponent): x = int32 2^exponent, the largest magnitude just below 2^24, the exponent a 1-element int32 device tensor.
-    What a bfloat16 tensor holds is exact down to 2^-24 of its largest value, where the shifts that follow have long left it.
+    x is float32 from float32 sums: PstoShift takes the low half of the bits that it drops for its random number, so these have to be
+    the sum's own.  Eight significant bits in front of zeros (bfloat16) would round almost every fraction up.
     A gradient with NaN in it (a target outside the classes; the loss says so) becomes zero: nothing is learnt from it."""
-    m = torch.nan_to_num(x.abs().amax().float(), nan=0.0, posinf=0.0)
+    m = torch.nan_to_num(x.abs().amax(), nan=0.0, posinf=0.0)
     e = torch.frexp(m)[1]
     half = (24 - e) // 2
-    y = torch.nan_to_num(x.float(), nan=0.0, posinf=0.0, neginf=0.0) * _power(half) * _power(24 - e - half)
+    y = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0) * _power(half) * _power(24 - e - half)
     return torch.where(m > 0, y, 0.0).to(torch.int32), (e - 24).reshape(1).to(torch.int32)
 
 
@@ -72,8 +73,8 @@ class TiVocabHead(ti_torch.UpdateWeight):
             grad = torch.full((1,), 1.0 / max(1, act[..., 0].numel()), dtype=torch.float32, device=act.device)
         da = dw = None
         for share, state in d["_parts"]:
-            a, w = ops.vocab_backward(act, self.weight, exp, w_exp, state, grad if share == 1.0 else grad * share)
-            da, dw = (a, w) if da is None else (da.float() + a.float(), dw.float() + w.float())
+            a, w = ops.vocab_backward(act, self.weight, exp, w_exp, state, grad if share == 1.0 else grad * share, torch.float32)
+            da, dw = (a, w) if da is None else (da + a, dw + w)
         d["_parts"] = None
         if not self.weight.is_contiguous():
             self.weight = self.weight.contiguous()

@@ -111,3 +111,22 @@ def test_workspace_and_state_sizes():
     # the gradient's piece is bounded whatever the classes: two million of them need no 60 GB
     assert lib.niti_vocab_backward_workspace(256, 1024, 512, 1024, 8192, 1024, 2000000) < 2 << 30
     assert lib.niti_vocab_backward_workspace(256, 64, 512, 64, 0, 64, 10) == 0
+
+
+def test_float32_gradients_refusals_and_workspace():
+    from niti_amd import _lib
+    lib = _lib.lib()
+    buf = (C.c_char * 65536)()
+    p = C.addressof(buf) + (-C.addressof(buf)) % 16
+
+    def backward(state=p, weight=p, weights=4, da=p, dw=p, t=1.0, ws=None, top=1):
+        return lib.niti_vocab_backward_i8_f32(p, 64, p, 64, p, p, 4, 64, 9, top, t, state, weight, weights, da, dw, ws, 0, None)
+
+    assert backward(state=None) == 1 and backward(da=None) == 1 and backward(dw=None) == 1 and backward(weights=3) == 1
+    assert backward(da=p + 4) == 1 and backward(dw=p + 8) == 1 and backward(t=-1.0) == 1 and backward(top=0) == 1
+    assert backward() == 3
+    # the sums of both gradients pass through it
+    size = (256, 64, 512, 64, 10, 64, 1000)
+    assert lib.niti_vocab_backward_f32_workspace(*size) >= lib.niti_vocab_backward_workspace(*size) > 0
+    assert lib.niti_vocab_backward_f32_workspace(*size) >= 4 * 64 * (10 + 1000)
+    assert lib.niti_vocab_backward_f32_workspace(256, 64, 512, 64, 0, 64, 10) == 0
