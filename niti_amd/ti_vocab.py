@@ -86,8 +86,11 @@ class TiVocabHead(ti_torch.UpdateWeight):
         self.grad, self.grad_shift = ops.grad_update(
             g, self.weight, ops.absmax_i32(g), ti_torch.GRAD_BITWIDTH, method, ti_torch.DIV_MODE, ti_torch.BW_MODE,
             ti_torch._rand_bits_like(g) if method == "sto" else None, want_grad=self.keep_grad, exp_a=g_exp, exp_out=self.grad_exp)
-        err, err_exp = _fixed_point(da)
-        y, _, exp_out = ti_torch._requant(err, ti_torch.BITWIDTH, ti_torch.ERROR_ROUND_METHOD, exp_a=err_exp, want_exp=True)
+        if da.numel() == 0:      # no rows
+            y, exp_out = torch.empty(da.shape, dtype=torch.int8, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+        else:
+            err, err_exp = _fixed_point(da)
+            y, _, exp_out = ti_torch._requant(err, ti_torch.BITWIDTH, ti_torch.ERROR_ROUND_METHOD, exp_a=err_exp, want_exp=True)
         self.err_exp = exp_out
         return y, exp_out
 

@@ -143,3 +143,17 @@ def test_mean_update_is_the_gradient(dev, monkeypatch):
         print("2^%d: %d weights, %.4f" % (i, count, off), flush=True)
         assert abs(off) <= 3.0 / count ** 0.5 + 2.0 ** -8 + 2.0 ** -9.9 * float(bound[at].mean())
     assert asked >= 4
+
+
+@pytest.mark.parametrize("shape", [(0, 96), (2, 0, 96)])
+def test_layer_without_rows(dev, shape):
+    from niti_amd.ti_vocab import TiVocabHead
+    head = TiVocabHead(96, 700)
+    before = head.weight.clone()
+    act = torch.empty(shape, dtype=torch.int8, device=dev)
+    target = torch.empty(shape[:-1], dtype=torch.int64, device=dev)
+    teacher = (torch.empty(shape[:-1] + (4,), device=dev), torch.empty(shape[:-1] + (4,), dtype=torch.int64, device=dev))
+    for what in ({"target": target}, {"teacher": teacher}, {"target": target, "teacher": teacher}):
+        assert head.forward((act, -5), **what).shape == shape[:-1]
+        err, exp = head.backward()
+        assert err.shape == shape and err.dtype == torch.int8 and exp.shape == (1,) and torch.equal(head.weight, before)

@@ -101,3 +101,16 @@ def test_what_bfloat16_would_give():
         mean[dtype] = y.double().mean(1) - dw.mean(1) / unit
     assert float(mean[torch.float32][:-1].abs().max()) <= TOLERANCE
     assert bool((mean[torch.bfloat16][:7] > torch.tensor([0.05, 0.1, 0.2, 0.4, 0.4, 0.15, 0.3])).all())
+
+
+@pytest.mark.parametrize("shape", [(0, 12), (0, 3, 12), (3, 0, 12)])
+def test_no_rows(head_on_cpu, shape):
+    """A batch of none is a step like any other: nothing is learnt, the error has the input's shape."""
+    head = head_on_cpu(torch.zeros(shape, dtype=torch.float64), torch.zeros((5, 12), dtype=torch.float64))
+    loss = head.forward((torch.empty(shape, dtype=torch.int8), -5), target=torch.empty(shape[:-1], dtype=torch.int64))
+    assert loss.shape == shape[:-1]
+    err, exp = head.backward()
+    assert err.shape == shape and err.dtype == torch.int8 and exp.dtype == torch.int32 and exp.shape == (1,)
+    assert bool((head.weight == 0).all())
+    with pytest.raises(RuntimeError, match="forward"):
+        head.backward()
