@@ -103,7 +103,7 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   for (int j = lane; j < top; j += 64) {
     const long long at = row * top + j;
     const int c = vocab_target(a.targets, at, a.classes);
-    const float given = a.value == nullptr ? 0.0f : teacher_value(a, at) / a.t;
+    const float given = a.value == nullptr ? 0.0f : teacher_value(a, at);
     if (c == -2) bad = true;
     cls[j] = c < 0 ? -1 : c;
     const float v = c < 0 ? -INFINITY : given;
@@ -141,7 +141,8 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   float norm = 0.0f;
   for (int j = lane; j < top; j += 64) {
     const float v = q[j];
-    const float e = v == -INFINITY ? 0.0f : expf(v - vmax);
+    // divided by T behind the difference: a type's lowest value over a T below 1 is no float32 number any more, its difference from another is
+    const float e = v == -INFINITY ? 0.0f : expf((v - vmax) / a.t);
     q[j] = e;
     norm += e;
   }
