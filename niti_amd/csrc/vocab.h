@@ -90,6 +90,24 @@ __device__ inline int wave_most(int v) {
 __device__ inline float wave_add(float v) {
   return __int_as_float(wave_fold(0, __float_as_int(v), [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); }));
 }
+// in 64 bits: the two halves move together
+template <int CTRL, int MASK>
+__device__ inline double dpp_take(double v) {
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  const int lo = dpp_take<CTRL, MASK>(0, static_cast<int>(b)), hi = dpp_take<CTRL, MASK>(0, static_cast<int>(b >> 32));
+  return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo)));
+}
+__device__ inline double wave_add(double v) {
+  v += dpp_take<0x111, 0xf>(v);
+  v += dpp_take<0x112, 0xf>(v);
+  v += dpp_take<0x114, 0xf>(v);
+  v += dpp_take<0x118, 0xf>(v);
+  v += dpp_take<0x142, 0xa>(v);
+  v += dpp_take<0x143, 0xc>(v);
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v));
+  const int lo = __builtin_amdgcn_readlane(static_cast<int>(b), 63), hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), 63);
+  return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo)));
+}
 __device__ inline float wave_most(float v) {
   return __int_as_float(wave_fold(__float_as_int(-INFINITY), __float_as_int(v), [](int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }));
 }

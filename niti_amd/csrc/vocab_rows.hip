@@ -79,7 +79,8 @@ __device__ inline float teacher_value(const VocabRows& a, long long i) {
 
 // A wavefront and workgroup per row.  All loads depend on nothing and go out together: pairs of the tiles, exponents, targets, their logits
 // and teacher's values; what the kernel takes is the way of these.  3.0 us for one row, 4.0 for 128, 20 for 8192 rows with 64
-// places.  Sums in 32 bits; a logit's distance from the largest and the logarithm of the sum meet in 64 bits.
+// places.  The tiles' sums, of 32 bits, are added in 64: a row that is all but sure of itself adds many small ones to one that is almost 1, and what they
+// come to is its loss.  A logit's distance from the largest and the logarithm of the sum meet in 64 bits.
 __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x;
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   for (int u = 0; u < kHeld; ++u) m = max(m, held[u].x);
   for (int i = lane + 64 * kHeld; i < a.tiles; i += 64) m = max(m, part[i].x);
   m = wave_most(m);
-  float sum = 0.0f;
+  double sum = 0.0;
 #pragma unroll
   for (int u = 0; u < kHeld; ++u)
     if (held[u].x != -2147483647 - 1) sum += __int_as_float(held[u].y) * exp2f(static_cast<float>(held[u].x - m) * kf);
@@ -129,12 +130,13 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
   }
   sum = wave_add(sum);
   int e2;
-  float mantissa = frexpf(sum, &e2);
-  if (mantissa < 0.70710678f) {
-    mantissa *= 2.0f;
+  double mantissa = frexp(sum, &e2);
+  if (mantissa < 0.70710678) {
+    mantissa *= 2.0;
     e2 -= 1;
   }
-  const double l2 = static_cast<double>(log2f(mantissa)) + e2;      // the float part is at most 1/2: a row that is sure of itself keeps its digits
+  // the float part is at most 1/2 and made of the distance from 1: a row that is sure of itself keeps its digits
+  const double l2 = 1.4426950408889634074 * static_cast<double>(log1pf(static_cast<float>(mantissa - 1.0))) + e2;
 
   vmax = wave_most(vmax);
   bad = __any(bad);

@@ -38,3 +38,25 @@ def test_teacher_values_over_a_temperature(dev, value, t):
     assert bool(torch.isfinite(want[0]).all())
     check_forward(got, want, t, 30.0)
     check_gradients(ops.vocab_backward(act, w, *e, got[2]), vo.backward(act, w, ea, ew, None, t, top_val=val, top_idx=idx), n, v)
+
+
+@pytest.mark.parametrize("n", [1, 40, 200])
+@pytest.mark.parametrize("v", [300000, 1000003])
+def test_rows_that_are_all_but_sure(dev, n, v):
+    """One class is ahead of many equal ones, and the loss is log(1 + (v - 1) 2^-31): what all the others come to.  Tiles' sums are float32 numbers.
+    The largest class's own, just above 1, may lose the other classes of its tile, at most 255 2^-31 < 2^-23: an addition's rounding is no more than
+    what is added.  The others keep 36 additions' 36 2^-24 of their value, their exponentials of 2^-31 31 ln 2 2^-23 + 2^-23, and the joined sum
+    and its logarithm 2^-22 of what is beside the 1: 2^-16 in all."""
+    from niti_amd import ops
+    f = 16
+    act = torch.zeros((n, f), dtype=torch.int8, device=dev)
+    act[:, 0] = 64
+    w = torch.zeros((v, f), dtype=torch.int8, device=dev)
+    best = 12345
+    w[best, 0] = 86                       # 5504 steps of 2^-8 ahead: e^-21.5 = 2^-31
+    target = torch.full((n,), best, dtype=torch.int64, device=dev)
+    loss, lse, _ = ops.vocab_loss(act, w, exp_of(-4, dev), exp_of(-4, dev), target)
+    want = float(torch.log1p(torch.tensor((v - 1) * float(torch.exp(torch.tensor(-21.5, dtype=torch.float64))), dtype=torch.float64)))
+    print(v, want, float(loss[0]), flush=True)
+    assert bool(((loss.double() - want).abs() <= 2.0 ** -23 + 2.0 ** -16 * want).all())
+    assert bool(((lse.double() - (21.5 + want)).abs() <= 2.0 ** -19).all())
