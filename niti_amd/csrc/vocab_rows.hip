@@ -3,8 +3,8 @@
 //   forward:  statistics of the logits per row and tile of classes and the logits of the targets (vocab.hip), then a wavefront per row
 //             joins them and leaves loss, logarithm of the denominator and what the backward pass wants to know
 //   backward: a piece of the classes after the other: the piece's softmax as 16-bit floats (vocab.hip), the targets' places
-//             overwritten with their gradient (known in 32 bits: a small difference p - q keeps its digits), both products in one launch,
-//             their slices added in another
+//             overwritten with their gradient (made in 32 bits: a difference p - q keeps what its rounding leaves, p - 1 its digits), both
+//             products in one launch, their slices added in another
 #include <math.h>
 
 #include "vocab.h"
@@ -169,7 +169,8 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
           all += q[i];
           if (i < j) first = false;      // one place speaks for all
         }
-      g = norm > 0.0f ? exp2f(static_cast<float>(behind)) - all / norm : 0.0f;
+      // p near 1 by its distance from 1: what p - 1 is of a row that is all but sure of itself has its own digits, not those that 1 leaves
+      if (norm > 0.0f) g = behind > -1.0 ? expm1f(static_cast<float>(kLn2 * behind)) + (norm - all) / norm : exp2f(static_cast<float>(behind)) - all / norm;
       if (coef != coef) g = coef;
     }
     *reinterpret_cast<int2*>(state + 4 + 2 * j) = make_int2(__float_as_int(g), first ? c : -1);

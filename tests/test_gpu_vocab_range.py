@@ -60,3 +60,33 @@ def test_rows_that_are_all_but_sure(dev, n, v):
     print(v, want, float(loss[0]), flush=True)
     assert bool(((loss.double() - want).abs() <= 2.0 ** -23 + 2.0 ** -16 * want).all())
     assert bool(((lse.double() - (21.5 + want)).abs() <= 2.0 ** -19).all())
+
+
+@pytest.mark.parametrize("kind", ["entropy", "distill"])
+@pytest.mark.parametrize("n", [1, 40, 200])
+def test_gradients_of_rows_that_are_all_but_sure(dev, kind, n):
+    """The same with 1 - p = 300000 e^-26.5 = 2^-20.  p - q of the target is within 2^-9.9 of its value like every other (see test_gpu_vocab.py),
+    beside what the largest class's own tile may lose, 255 of the 300000 others; where a product has one term that counts, it is the result's
+    error, with 2^-24 of the sum in float32."""
+    from niti_amd import ops
+    f, v, best = 16, 300000, 12345
+    act = torch.zeros((n, f), dtype=torch.int8, device=dev)
+    act[:, 0] = 64
+    w = torch.zeros((v, f), dtype=torch.int8, device=dev)
+    w[best, 0] = 106                      # 26.5
+    e = (exp_of(-4, dev), exp_of(-4, dev))
+    if kind == "entropy":
+        state = ops.vocab_loss(act, w, *e, torch.full((n,), best, dtype=torch.int64, device=dev))[2]
+    else:
+        idx = torch.tensor([best, 17, best], device=dev).repeat(n, 1)
+        state = ops.vocab_distill(act, w, *e, torch.tensor([1.0, -torch.inf, 1.0], device=dev).repeat(n, 1), idx)[2]
+    da, dw = ops.vocab_backward(act, w, *e, state, torch.full((1,), 1.0 / n, device=dev), torch.float32)
+    small = float(torch.exp(torch.tensor(-26.5, dtype=torch.float64)))
+    rest = (v - 1) * small / (1.0 + (v - 1) * small)
+    tol = 2.0 ** -9.9 + 255.0 / v + 2.0 ** -22
+    print(kind, n, rest, float(dw[best, 0]) / -4.0, flush=True)
+    assert abs(float(dw[best, 0]) / (-rest * 64 * 2.0 ** -4) - 1.0) <= tol
+    assert bool((da[:, 0].double() / (-rest * 106 * 2.0 ** -4 / n) - 1.0).abs().max() <= tol)
+    # a place of weight zero has its softmax
+    if kind == "distill":
+        assert abs(float(dw[17, 0]) / (small * 64 * 2.0 ** -4) - 1.0) <= 0.5 / 1.7      # 2^-38 is 1.7 of float16's last places here
