@@ -601,7 +601,9 @@ int niti_group_conv_i8_f32(const int8_t* x, const int8_t* w, float* y, int N, in
  * numbers finds none in bfloat16).  weight: `weights` = rows values, one for all, or null for 1.  The logits are computed again, a piece of the
  * classes at a time; the softmax of a piece, times 2^15, and weight[n] act, over a power of two, are held as float16.
  *
- * The workspaces depend on the operands' addresses through their alignment alone.
+ * The workspaces depend on the operands' addresses through their alignment alone.  The backward call's grows with the rows: 8 KiB each for a piece of the
+ * gradient (128 MiB up to 16384 rows), 2 bytes per row and feature for the activations' 16-bit copy, 4 for sums carried over the pieces; not with the classes,
+ * apart from a copy of weights that cannot be read in place.
  */
 enum { NITI_F32 = 0, NITI_BF16 = 1, NITI_F16 = 2 };
 size_t niti_vocab_state_words(int top);

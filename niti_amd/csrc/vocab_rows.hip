@@ -14,8 +14,13 @@ namespace {
 
 constexpr int kMaxFeatures = 65536;      // |s| <= 2^30: differences of two logits are int32
 constexpr long long kPieceMost = 1LL << 20;
-constexpr long long kPieceGrad = 64LL << 20;    // elements of the gradient's piece: 128 MiB, half of the last-level cache
-constexpr long long kPieceWide = 128LL << 20;   // elements of the weights' 16-bit copy
+// A piece of the classes: as many as leave the gradient at 128 MiB, half of the last-level cache, and the weights' 16-bit copy at 256 MiB, but 4096 at
+// least.  Rows are not cut: from 16384 on the gradient is 8 KiB of each, whatever the cache holds, and from 32768 features on the weights' copy 8 KiB of each
+// feature.  Every piece adds to all of d_act's float32 sums, so fewer classes cost more than they save: 131072 rows over 32000 classes 8.3 ms at
+// 256 features and 11.7 at 512 with 4096 classes, 14.8 and 17.1 with 512 and 1024.
+constexpr long long kPieceGrad = 64LL << 20;    // values
+constexpr long long kPieceWide = 128LL << 20;   // values
+constexpr long long kPieceLeast = 4096;         // classes
 
 long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
 
@@ -255,7 +260,7 @@ BackwardPlan backward_plan(const Matrix& a, const Matrix& w, int features, bool 
   p.part_pitch = round_up(features, 4);
   long long piece = kPieceGrad / a.rows;
   if (a.rows > 32 && piece > kPieceWide / features) piece = kPieceWide / features;
-  if (piece < 4096) piece = 4096;
+  if (piece < kPieceLeast) piece = kPieceLeast;
   if (piece > kPieceMost) piece = kPieceMost;
   piece = piece / 256 * 256;
   if (piece > round_up(w.rows, 8)) piece = round_up(w.rows, 8);
