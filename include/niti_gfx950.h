@@ -583,7 +583,8 @@ int niti_group_conv_i8_f32(const int8_t* x, const int8_t* w, float* y, int N, in
  * Losses over many classes, the logits kept nowhere.  No counterpart in the reference, whose loss (ti_loss.py:5-36) takes int8
  * logits that lie in memory.  act: [rows][features] int8, w: [classes][features] int8, rows act_pitch / w_pitch bytes apart (any
  * alignment; read in place where address and pitch are multiples of four bytes and the features of 16, the weights' of 4), exponents in
- * device memory; a logit is z = (act . w) 2^(exp_a + exp_w), the sum exact in int32 (features <= 65536).
+ * device memory; a logit is z = (act . w) 2^(exp_a + exp_w), the sum exact in int32 (features <= 65536).  Rows and weights less than 4 MiB apart, fewer than
+ * 2^26 rows; what needs a grid of 2^32 work-items and more is NITI_ERR_UNSUPPORTED.
  *
  * niti_vocab_entropy_i8: loss[n] = log sum_v exp(z[n,v]) - z[n,target[n]], lse[n] = log sum_v exp(z[n,v]) in float32.  target: int32
  * or int64 by target_bytes.  A row whose target is `ignored` has loss 0 and no gradient; any other target outside the classes

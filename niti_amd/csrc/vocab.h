@@ -67,6 +67,12 @@ __device__ inline int vocab_target(const VocabTargets& t, long long at, int clas
   return c >= 0 && c < classes ? static_cast<int>(c) : -2;
 }
 
+// A grid's work-items are counted in 32 bits.
+inline int check_grid(long long workgroups, int threads, const char* what) {
+  if (workgroups > 0xffffffffLL / threads) return fail(NITI_ERR_UNSUPPORTED, "%s: %lld workgroups of %d", what, workgroups, threads);
+  return NITI_OK;
+}
+
 // Sums and maxima over the wavefront by data-parallel moves (a scan inside each row of sixteen lanes, the row totals carried on), in every
 // lane: six moves of a few clocks where a shuffle through LDS is some hundred.
 template <int CTRL, int MASK>

@@ -1043,26 +1043,28 @@ long long logit_blocks(const VocabLogits& l) {
 }
 template <class T>
 int run_stats(const VocabLogits& l, const VocabStats& s, const VocabTargets& targets, hipStream_t stream) {
-  if (const int rc = with_lds<vocab_stats_kernel<T>>(T::kLdsLogits, "vocab_stats")) return rc;
   // beside the tiles they have the tiles' LDS, hence few wavefronts of a unit: many go out in a launch of their own
   const long long units = static_cast<long long>(l.rows) * ((targets.top + kPlaces - 1) / kPlaces);
   const bool apart = units > 4096;
+  const long long dots = apart ? 0 : ((units + T::kWaves - 1) / T::kWaves + 7) / 8 * 8;
+  const long long blocks = logit_blocks<T>(l) + dots;
+  if (const int rc = check_grid(blocks, T::kThreads, "vocab_stats")) return rc;
+  if (const int rc = check_grid((units + 3) / 4, 256, "vocab_dots")) return rc;
+  if (tiles_of(l.classes, l.rows, T::TI, T::TJ) > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: 2^31 tiles and more");
+  if (const int rc = with_lds<vocab_stats_kernel<T>>(T::kLdsLogits, "vocab_stats")) return rc;
   if (apart) {
-    if (units > 4LL * 0x7fffffff) return fail(NITI_ERR_UNSUPPORTED, "vocab_dots: %lld groups of places", units);
     hipLaunchKernelGGL(vocab_dots_kernel, dim3(static_cast<unsigned>((units + 3) / 4)), dim3(256), 0, stream, l, targets);
     if (const int rc = check_launch("vocab_dots")) return rc;
   }
-  const long long dots = apart ? 0 : ((units + T::kWaves - 1) / T::kWaves + 7) / 8 * 8;
-  const long long blocks = logit_blocks<T>(l) + dots;
-  if (blocks > 0x7fffffffLL || tiles_of(l.classes, l.rows, T::TI, T::TJ) > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_stats: %lld workgroups", blocks);
   hipLaunchKernelGGL(vocab_stats_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(T::kThreads), T::kLdsLogits, stream, l, s, targets, static_cast<int>(dots));
   return check_launch("vocab_stats");
 }
 template <class T>
 int run_grad(const VocabLogits& l, const VocabGrad& g, hipStream_t stream) {
-  if (const int rc = with_lds<vocab_grad_kernel<T>>(T::kLdsLogits, "vocab_grad")) return rc;
   const long long blocks = logit_blocks<T>(l) + (g.widen_a.blocks + g.widen_w.blocks + 7) / 8 * 8;
-  if (blocks > 0x7fffffffLL || tiles_of(l.classes, l.rows, T::TI, T::TJ) > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_grad: %lld workgroups", blocks);
+  if (const int rc = check_grid(blocks, T::kThreads, "vocab_grad")) return rc;
+  if (tiles_of(l.classes, l.rows, T::TI, T::TJ) > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_grad: 2^31 tiles and more");
+  if (const int rc = with_lds<vocab_grad_kernel<T>>(T::kLdsLogits, "vocab_grad")) return rc;
   hipLaunchKernelGGL(vocab_grad_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(T::kThreads), T::kLdsLogits, stream, l, g);
   return check_launch("vocab_grad");
 }
@@ -1070,9 +1072,9 @@ template <class TA, class TW>
 int run_sums(const VocabSums& a, const VocabSums& w, hipStream_t stream) {
   constexpr int kLdsA = TA::kRings * TA::RING * (stage_bytes(TA::TI, TA::TI == 256 ? kSlow16 : kSlow8) + stage_bytes(TA::TJ, kFast)), kOutA = 2 * TA::TI * TA::TJ;
   constexpr int kMostA = kLdsA > kOutA ? kLdsA : kOutA, kLds = kMostA > TW::kLds ? kMostA : TW::kLds;
-  if (const int rc = with_lds<vocab_sums_kernel<TA, TW>>(kLds, "vocab_sums")) return rc;
   const long long na = (tiles_of(a.ni, a.nj, TA::TI, TA::TJ) * a.slices + 7) / 8 * 8, nw = tiles_of(w.ni, w.nj, TW::TI, TW::TJ) * w.slices;
-  if (na + nw > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_sums: %lld tiles", na + nw);
+  if (const int rc = check_grid(na + nw, TA::kThreads, "vocab_sums")) return rc;
+  if (const int rc = with_lds<vocab_sums_kernel<TA, TW>>(kLds, "vocab_sums")) return rc;
   hipLaunchKernelGGL((vocab_sums_kernel<TA, TW>), dim3(static_cast<unsigned>(na + nw)), dim3(TA::kThreads), kLds, stream, a, w, static_cast<int>(na));
   return check_launch("vocab_sums");
 }
@@ -1209,7 +1211,7 @@ int launch_vocab_sums(VocabTile t, const VocabSums& a, const VocabSums& w, hipSt
 int launch_vocab_join(const VocabSums* a, const VocabSums* w, hipStream_t stream) {
   const auto blocks = [](const VocabSums* s) { return s == nullptr ? 0 : (static_cast<long long>((s->ni + 3) / 4) * s->nj + 255) / 256; };
   const long long na = blocks(a), nw = blocks(w);
-  if (na + nw > 0x7fffffffLL) return fail(NITI_ERR_UNSUPPORTED, "vocab_join: %lld workgroups", na + nw);
+  if (const int rc = check_grid(na + nw, 256, "vocab_join")) return rc;
   hipLaunchKernelGGL(vocab_join_kernel, dim3(static_cast<unsigned>(na + nw)), dim3(256), 0, stream, a != nullptr ? *a : *w, w != nullptr ? *w : *a, static_cast<int>(na));
   return check_launch("vocab_join");
 }

@@ -13,6 +13,7 @@ namespace niti {
 namespace {
 
 constexpr int kMaxFeatures = 65536;      // |s| <= 2^30: differences of two logits are int32
+constexpr int kMaxRows = (1 << 26) - 1;  // a wavefront each in one launch
 constexpr long long kPieceMost = 1LL << 20;
 // A piece of the classes: as many as leave the gradient at 128 MiB, half of the last-level cache, and the weights' 16-bit copy at 256 MiB, but 4096 at
 // least.  Rows are not cut: from 16384 on the gradient is 8 KiB of each, whatever the cache holds, and from 32768 features on the weights' copy 8 KiB of each
@@ -287,6 +288,7 @@ int pad_rows(Matrix* a, bool copy_a, int8_t* to_a, Matrix* w, bool copy_w, int8_
     return VocabPad{m.p, m.pitch, to, m.rows, copy ? static_cast<int>((m.rows * ((features + 15) / 16) + 255) / 256) : 0};
   };
   const VocabPad pa = pad(*a, copy_a, to_a), pw = pad(*w, copy_w, to_w);
+  if (const int rc = check_grid(static_cast<long long>(pa.blocks) + pw.blocks, 256, "vocab_pad")) return rc;
   hipLaunchKernelGGL(vocab_pad_kernel, dim3(static_cast<unsigned>(pa.blocks) + static_cast<unsigned>(pw.blocks)), dim3(256), 0, stream, pa, pw, features);
   if (copy_a) *a = Matrix{to_a, round_up(features, 16), a->rows, static_cast<int>(round_up(features, 16))};
   if (copy_w) *w = Matrix{to_w, round_up(features, 16), w->rows, static_cast<int>(round_up(features, 16))};
@@ -303,6 +305,7 @@ int check_operands(const char* who, const int8_t* act, long long act_pitch, cons
     return fail(NITI_ERR_INVALID_ARG, "%s: rows=%d features=%d classes=%d top=%d", who, rows, features, classes, top);
   if (act_pitch < features || w_pitch < features) return fail(NITI_ERR_INVALID_ARG, "%s: rows of %lld and %lld bytes hold no %d features", who, act_pitch, w_pitch, features);
   if (features > kMaxFeatures) return fail(NITI_ERR_UNSUPPORTED, "%s: %d features (at most %d)", who, features, kMaxFeatures);
+  if (rows > kMaxRows) return fail(NITI_ERR_UNSUPPORTED, "%s: %d rows (at most %d)", who, rows, kMaxRows);
   if (act_pitch >= (1LL << 22) || w_pitch >= (1LL << 22)) return fail(NITI_ERR_UNSUPPORTED, "%s: rows 4 MiB or more apart", who);
   if (top > kVocabTopMost) return fail(NITI_ERR_UNSUPPORTED, "%s: lists of %d (at most %d)", who, top, kVocabTopMost);
   return NITI_OK;
@@ -344,6 +347,7 @@ int backward(const int8_t* act, long long act_pitch, const int8_t* w, long long 
   if (!aligned16(state) || !aligned16(d_act) || !aligned16(d_w)) return fail(NITI_ERR_INVALID_ARG, "%s: state or result not 16-byte aligned", who);
   Matrix a{act, act_pitch, rows, features}, b{w, w_pitch, classes, features};
   const BackwardPlan p = backward_plan(a, b, features, f32);
+  if (const int rc = check_grid((static_cast<long long>(rows) * ((features + 3) / 4) + 255) / 256, 256, "vocab_join")) return rc;      // before anything runs
   if (workspace == nullptr || workspace_bytes < p.bytes || !aligned16(workspace))
     return fail(NITI_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, got %zu", who, p.bytes, workspace_bytes);
   char* const ws = static_cast<char*>(workspace);
@@ -371,6 +375,7 @@ int backward(const int8_t* act, long long act_pitch, const int8_t* w, long long 
     if (const int rc = launch_vocab_grad(tile, l, VocabGrad{state, vocab_state_words(top), targets ? top : 0, first, grad, p.piece, widen_a, widen_w}, st)) return rc;
     if (!targets) {
       const long long places = static_cast<long long>(rows) * top;
+      if (const int rc = check_grid((places + 255) / 256, 256, "vocab_targets")) return rc;
       hipLaunchKernelGGL(vocab_targets_kernel, dim3(static_cast<unsigned>((places + 255) / 256)), dim3(256), 0, st, state, rows, top, first, here, grad, p.piece);
       if (const int rc = check_launch(who)) return rc;
     }

@@ -1,4 +1,6 @@
 """What a call of the losses over many classes takes, without a GPU: memory, limits."""
+import ctypes as C
+
 import pytest
 
 
@@ -17,3 +19,22 @@ def test_the_backward_workspace_of_many_rows(lib, rows, features, classes):
     row = 8192 + 6 * features
     short, wide = lib.niti_vocab_backward_workspace(*size), lib.niti_vocab_backward_f32_workspace(*size)
     assert rows * 2 * (3000 + features) <= short <= wide <= rows * row + (769 << 20)
+
+
+def test_calls_beyond_a_grid_are_refused(lib):
+    """By the check of the arguments, not by a launch that fails when others have run: NITI_ERR_UNSUPPORTED."""
+    buf = (C.c_char * 4096)()
+    p = C.addressof(buf) + (-C.addressof(buf)) % 16
+
+    def forward(rows, features, classes):
+        return lib.niti_vocab_entropy_i8(p, features, p, features, p, p, rows, features, classes, p, 8, -100, p, p, p, p, 1 << 60, None)
+
+    def backward(rows, features, classes):
+        return lib.niti_vocab_backward_i8(p, features, p, features, p, p, rows, features, classes, 1, 1.0, p, None, 0, p, p, p, 1 << 60, None)
+
+    for call in (forward, backward):
+        assert call(1 << 26, 64, 100) == 2 and b"rows" in lib.niti_last_error()
+        assert call(0x7fffffff, 64, 100) == 2
+    assert backward(1 << 25, 1024, 100) == 2 and b"workgroups" in lib.niti_last_error()
+    # 2^30 tiles of 256 work-items: a 32-bit number of workgroups, none of work-items
+    assert forward(1 << 20, 64, 1 << 24) == 2 and b"workgroups" in lib.niti_last_error()
