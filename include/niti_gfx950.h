@@ -629,6 +629,13 @@ int niti_vocab_backward_i8_f32(const int8_t* act, int64_t act_pitch, const int8_
  * MEASUREMENT ONLY - not part of the boundary a reference checkout binds to; nothing in the layers calls it.
  * ================================================================================================================== */
 /*
+ * What a call of the losses over many classes takes: plan[6] = tile of the forward call's logits, of the first piece's gradient and of the sums (0: 256 x 256,
+ * 1: 128 x 128, 2: 64 x 64, 3: sums of few rows, 4: 32 rows, 5: 128 x 128 in one buffer, 6 and 7: wavefronts with stages of their own, 64 x 64 and 64 x 32),
+ * classes of a piece, parts that the activations' and the weights' sums are cut into.  Tests see by it that their sizes reach every kernel.
+ */
+int niti_vocab_plan(int rows, int features, int classes, int* plan);
+
+/*
  * Measurement aid, no counterpart in the reference: a register-resident int8 MFMA loop (v_mfma_i32_32x32x32_i8, no LDS
  * and no memory traffic inside the loop) over operand fragments read once from `operands` (operand_bytes >= 128,
  * 16-byte aligned).  `workgroups` x 8 wavefronts each run `iters` rounds of 12 MFMAs = iters * 12 * 65536 int8

@@ -101,6 +101,7 @@ SIGNATURES = {
     "niti_vocab_state_words": (_sz, [_i]),
     "niti_vocab_forward_workspace": (_sz, [_vp, _i64, _vp, _i64] + [_i] * 3),
     "niti_vocab_backward_workspace": (_sz, [_vp, _i64, _vp, _i64] + [_i] * 3),
+    "niti_vocab_plan": (_i, [_i, _i, _i, _vp]),
     "niti_vocab_backward_f32_workspace": (_sz, [_vp, _i64, _vp, _i64] + [_i] * 3),
     "niti_vocab_entropy_i8": (_i, [_vp, _i64, _vp, _i64, _vp, _vp] + [_i] * 3 + [_vp, _i, _i64, _vp, _vp, _vp, _vp, _sz, _vp]),
     "niti_vocab_distill_i8": (_i, [_vp, _i64, _vp, _i64, _vp, _vp] + [_i] * 3 + [_vp, _i, _vp, _i, _i, C.c_float, _vp, _vp, _vp, _vp, _sz, _vp]),

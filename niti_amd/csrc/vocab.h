@@ -163,6 +163,7 @@ struct VocabSums {           // out[j][i] = sum_k x[i][k] y[j][k] in float
 // The tiles of a launch (vocab.hip): 256 x 256; 128 x 128 two to a unit; 64 x 64; short, the sums of few rows (64 x 64 for the activations, one
 // buffer of 128 x 128 for the weights); 32 rows; 128 x 128 in one buffer, four to a unit; 64 x 64 and, of 32 rows, 64 x 32 whose wavefronts take
 // stages of their own
+// (niti_vocab_plan gives their numbers out)
 enum VocabTile { kVocabLarge, kVocabMiddle, kVocabSmall, kVocabShort, kVocabFew, kVocabQuad, kVocabSmallApart, kVocabFewApart };
 VocabTile vocab_logits_tile(int rows, int features, int classes);
 int vocab_stats_tiles(VocabTile t, int classes);    // pairs that launch_vocab_stats leaves of a row

@@ -421,6 +421,19 @@ extern "C" size_t niti_vocab_backward_f32_workspace(const int8_t* act, int64_t a
   return backward_plan(Matrix{act, act_pitch, rows, features}, Matrix{w, w_pitch, classes, features}, features, true).bytes;
 }
 
+extern "C" int niti_vocab_plan(int rows, int features, int classes, int* plan) {
+  clear_error();
+  if (plan == nullptr || rows <= 0 || features <= 0 || classes <= 0) return fail(NITI_ERR_INVALID_ARG, "vocab_plan: rows=%d features=%d classes=%d", rows, features, classes);
+  const BackwardPlan p = backward_plan(Matrix{nullptr, features, rows, features}, Matrix{nullptr, features, classes, features}, features, false);
+  plan[0] = vocab_logits_tile(rows, features, classes);
+  plan[1] = vocab_logits_tile(rows, features, static_cast<int>(p.piece < classes ? p.piece : classes));
+  plan[2] = p.tile;
+  plan[3] = static_cast<int>(p.piece);
+  plan[4] = p.slices_a;
+  plan[5] = p.slices_w;
+  return NITI_OK;
+}
+
 extern "C" int niti_vocab_entropy_i8(const int8_t* act, int64_t act_pitch, const int8_t* w, int64_t w_pitch, const int32_t* exp_a, const int32_t* exp_w, int rows,
                                      int features, int classes, const void* target, int target_bytes, int64_t ignored, float* loss, float* lse, int32_t* state,
                                      void* workspace, size_t workspace_bytes, void* stream) {

@@ -38,3 +38,36 @@ def test_calls_beyond_a_grid_are_refused(lib):
     assert backward(1 << 25, 1024, 100) == 2 and b"workgroups" in lib.niti_last_error()
     # 2^30 tiles of 256 work-items: a 32-bit number of workgroups, none of work-items
     assert forward(1 << 20, 64, 1 << 24) == 2 and b"workgroups" in lib.niti_last_error()
+
+
+def _plan(lib, rows, features, classes):
+    plan = (C.c_int * 6)()
+    assert lib.niti_vocab_plan(rows, features, classes, plan) == 0
+    return list(plan)
+
+
+def test_the_sizes_of_the_gpu_tests_reach_every_kernel(lib):
+    """The rules that choose a tile are refitted now and then: none may lose its test by it."""
+    from vocab_sizes import SIZES, TILES
+    plans = [((kind, n, f, v, k), _plan(lib, n, f, v)) for kind, n, f, v, k in SIZES]
+    for kind in ("entropy", "distill"):
+        seen = [p for (what, *_), p in plans if what == kind]
+        of_logits = set(TILES) - {"short"}       # a tile of the sums alone
+        assert {TILES[p[2]] for p in seen} >= {"large", "middle", "short", "small_apart"}, kind
+        assert {TILES[p[0]] for p in seen} >= {"large", "middle", "small", "quad"} and {TILES[p[1]] for p in seen} >= {"large", "middle", "small", "quad"}, kind
+    assert {TILES[p[0]] for _, p in plans} == of_logits == {TILES[p[1]] for _, p in plans}
+    assert {TILES[p[2]] for _, p in plans} == set(TILES)
+    large = TILES.index("large")
+    tiles = [-(-v // 256) * -(-n // 256) for (_, n, _, v, _), p in plans if p[0] == large]
+    assert min(tiles) > 256 and max(tiles) > 4 * 256                                                      # in turn, and more than twice
+    assert any(p[2] == large and p[3] < v for (_, _, _, v, _), p in plans)                                # sums over several pieces
+    assert any(p[2] == large and p[4] > 1 for _, p in plans) and any(p[5] > 1 for _, p in plans)          # cut reductions
+    for name, most in (("large", 0), ("middle", 32), ("quad", 32), ("small_apart", 32), ("few_apart", 128)):   # longer lists than the tile writes
+        assert any(p[1] == TILES.index(name) and k > most for (kind, _, _, _, k), p in plans if kind == "distill"), name
+
+
+def test_plan_refusals(lib):
+    plan = (C.c_int * 6)()
+    for wrong in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (-1, 1, 1)):
+        assert lib.niti_vocab_plan(*wrong, plan) == 1
+    assert lib.niti_vocab_plan(1, 1, 1, None) == 1
