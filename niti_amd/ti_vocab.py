@@ -25,8 +25,8 @@ def _fixed_point(x):
     m = torch.nan_to_num(x.abs().amax(), nan=0.0, posinf=0.0)
     e = torch.frexp(m)[1]
     half = (24 - e) // 2
-    y = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0) * _power(half) * _power(24 - e - half)
-    return torch.where(m > 0, y, 0.0).to(torch.int32), (e - 24).reshape(1).to(torch.int32)
+    y = torch.nan_to_num(x, nan=0.0, posinf=0.0, neginf=0.0) * torch.where(m > 0, _power(half), 0.0) * _power(24 - e - half)
+    return y.to(torch.int32), (e - 24).reshape(1).to(torch.int32)
 
 
 class TiVocabHead(ti_torch.UpdateWeight):
