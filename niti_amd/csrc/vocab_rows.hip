@@ -141,8 +141,9 @@ __global__ __launch_bounds__(64) void vocab_rows_kernel(const VocabRows a) {
     mantissa *= 2.0;
     e2 -= 1;
   }
-  // the float part is at most 1/2 and made of the distance from 1: a row that is sure of itself keeps its digits
-  const double l2 = 1.4426950408889634074 * static_cast<double>(log1pf(static_cast<float>(mantissa - 1.0))) + e2;
+  // the float part is at most 1/2, and what the mantissa has beyond float counts by the logarithm's slope at 1: a row that is sure of itself keeps its digits
+  const float rounded = static_cast<float>(mantissa);
+  const double l2 = 1.4426950408889634074 * (mantissa - rounded) + log2f(rounded) + e2;
 
   vmax = wave_most(vmax);
   bad = __any(bad);
