@@ -10,9 +10,9 @@
 //            XOR-swizzled by the step
 //   kSlow8   the same of int8 columns, transposed by ds_read_b64_tr_b8 and made 16-bit floats in registers (exact)
 //
-// What bounds the 256 x 256 tile is the matrix units' power more than its schedule: over 8192 x 8192 x 4096 the statistics, a piece of
-// the gradient and the two sums took 264, 235, 430 and 390 us on data and 189, 180, 312 and 297 us, in the same code, on zeros.  What was
-// measured on the way there, as sums of one gradient and of the other: loads issued all at once behind the barrier 464 and 437, spread
+// What bounds the 256 x 256 tile is the clock that its power leaves: over 8192 x 8192 x 4096 the statistics, a piece of the gradient and the two
+// sums took 264, 235, 430 and 390 us on data and 189, 180, 312 and 297 us, in the same code, on zeros, and by the counters as many clocks, of 1.83 GHz
+// (gradient 2.00) and 2.3 (2.4).  In 65, 51 and 68 % of the clocks the matrix units are busy.  What was measured on the way there, as sums of one gradient and of the other: loads issued all at once behind the barrier 464 and 437, spread
 // over the products of half a stage 427 and 393; with the loads left out 381 and 359, with products alone 335 and 308; two phases of half
 // the rows with a barrier each 446 and 407; four wavefronts of 128 x 128, whose sums move between register files, 635 and 589.
 #include "lds_asm.h"
@@ -670,7 +670,7 @@ __device__ inline void stats_of(const VocabLogits& l, const VocabStats& st, cons
   }
 }
 
-// Bound by the products: 8192 rows of 4096 features over 131072 classes 3.14 - 3.37 ms on two cards, 2.6 - 2.8 POP/s; few rows by the weights' way: 16 rows over
+// Bound by the products: 8192 rows of 4096 features over 131072 classes 3.14 - 3.37 ms on three cards, 2.6 - 2.8 POP/s; few rows by the weights' way: 16 rows over
 // 32000 classes of 4096 21 us, 131 MB at 6.2 TB/s called again and again, partly out of the last-level cache.  A pair per row and tile of
 // classes is all that leaves.
 // Statistics of the tiles, or - the first `others` workgroups, a multiple of eight - the targets' logits, which depend on nothing else
@@ -1142,8 +1142,9 @@ int launch_vocab_grad(VocabTile t, const VocabLogits& l, const VocabGrad& g, hip
 namespace {
 // What a workgroup of the sums takes, in us: per stage and beside them, with as many of its kind on the device as `slots`.  Fitted, with
 // the two terms of the parts' adding below, to the times of every tile and cut for 35 sizes (1 to 8192 rows, 64 to 4096 features, 100 to 60032
-// classes, some 1400 combinations): what the plan picks is at most 4 % off the best of them.  The wavefronts' own stages (the two ...Apart)
-// were fitted later, to 26 sizes of 1 to 400 rows: 16 x 512 over 2000 7.6 us (128 x 32 13.6), 128 x 512 over 1000 7.0 (8.7).
+// classes, some 1400 combinations): for those sizes what the plan picks is at most 4 % off the best of them.  The wavefronts' own stages (the two ...Apart)
+// were fitted later, to 26 sizes of 1 to 400 rows, most within 10 % of the best: 16 x 512 over 2000 7.6 us (128 x 32 13.6), 128 x 512 over 1000 7.0 (8.7), but
+// 32 x 64 over 4000 10.8 for 7.8.
 struct SumsCost {
   int ti, tj, slots;
   double stage, fixed;

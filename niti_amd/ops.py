@@ -351,7 +351,7 @@ def vocab_loss(act, w, exp_a, exp_w, target, ignore_index=-100):
     """Softmax cross entropy of a classifier over many classes, its logits kept nowhere: act [..., F] int8, w [V,F] int8, exponents
     as 1-element int32 tensors, z = (act @ w^T) 2^(exp_a + exp_w).  target [...] int64 or int32; ``ignore_index``: no target, the
     row's loss is 0 and it has no gradient; any other target outside the classes makes the row's loss (and the gradients) NaN.  Rows
-    may be spaced apart (a slice of a wider tensor).  Returns (loss [...], log sum exp z [...], state), float32, one per row."""
+    may be spaced apart, less than 4 MiB (a slice of a wider tensor).  Returns (loss [...], log sum exp z [...], state), float32, one per row."""
     loss, lse, rows = L.host().vocab_forward(act, w, exp_a, exp_w, None, target, ignore_index, 1.0)
     return loss, lse, VocabState(rows, 1, 1.0)
 
@@ -369,8 +369,8 @@ def vocab_backward(act, w, exp_a, exp_w, state, grad=None, dtype=torch.bfloat16)
     """Gradients of sum(grad * loss) of the vocab_loss or vocab_distill call that returned ``state``, with respect to the real values
     act 2^exp_a and w 2^exp_w: (d_act like act, d_w [V,F]) as ``dtype``, bfloat16 or float32, summed in float32.  ``grad``: float32, one value or one per
     row; None: 1.  The softmax is computed again, a piece of the classes at a time, and held as float16 (scaled: eleven bits down
-    to 2^-29), so the gradients carry three roundings more than the sums: that of p - q to eleven bits, d_w's of grad act to
-    eleven (fewer where a row's grad is below 2^-22 of the largest), and a bfloat16 result's to eight.  What rounds the result itself, and
+    to 2^-29, fewer to 2^-39, below 2^-40 nothing), so the gradients carry three roundings more than the sums: that of p - q to eleven bits,
+    d_w's of grad act to eleven (fewer where a row's grad is below 2^-22 of the largest, and in the end none), and a bfloat16 result's to eight.  What rounds the result itself, and
     by its low bits (PstoShift), wants float32."""
     if dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError("vocab_backward: gradients as bfloat16 or float32")
